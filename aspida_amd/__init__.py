@@ -47,6 +47,7 @@ def load(path=None):
         raise RuntimeError(f"libaspidagpu.so not found at {p}: build it with `python -m aspida_amd.build`")
     L = ctypes.CDLL(p, mode=ctypes.RTLD_GLOBAL)
     P, I, LG, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
+    LL = ctypes.c_longlong
     sig = {
         "aspida_gpu_matvec": (None, [P, LG, I, I, I, P, P]),
         "aspida_gpu_matmul": (None, [P, LG, I, I, I, I, P, P]),
@@ -75,6 +76,17 @@ def load(path=None):
         "aspida_moe_packed_work_bytes": (LG, [I, I, I, I]),
         "aspida_moe_pack_experts_dev": (I, [I, P, LG, I, I, I, P, P]),
         "aspida_moe_experts_packed_dev": (I, [P, I, I, I, I, I, P, P, P, P, I, P, I, P, P, P, P, P, P, P]),
+        "aspida_rope_create": (P, [P]),
+        "aspida_rope_table": (I, [P, P, P]),
+        "aspida_rope_destroy": (None, [P]),
+        "aspida_rope_dev": (I, [P, I, P, LL, I, I, I, P, I, P, LL, P]),
+        "aspida_kv4_page_bytes": (LL, [I, I]),
+        "aspida_kv4_append_dev": (I, [P, I, P, LL, P, LL, I, I, P, P, P, P, P]),
+        "aspida_kv4_read_dev": (I, [P, I, I, I, P, P, P, LL, P, LL, P]),
+        "aspida_kv4_attn_work_bytes": (LL, [P, I, I, I, I]),
+        "aspida_kv4_attn_dev": (I, [P, I, P, LL, I, I, I, P, I, P, F, I, P, LL, P, P, P]),
+        "aspida_kv4_weigh_dev": (I, [P, I, P, LL, I, I, I, P, I, P, F, I, P, P, P, LL, P]),
+        "aspida_kv4_evict_dev": (I, [P, I, P, P, LL, I, I, I, P, P, P, P, P]),
         "aspida_kq_chain_create": (P, [P, I]),
         "aspida_kq_chain_run": (I, [P, P]),
         "aspida_kq_chain_check": (I, [P]),
@@ -359,6 +371,51 @@ class DeviceOps:
                                                         shared_gate_inp or 0, work, y, stream),
                  "aspida_moe_experts_packed_dev")
 
+    def rope(self, rope, type, x, x_stride, n_tok, n_heads, head_dim, pos, y, y_stride, stream=0, inverse=False):
+        """y = x [n_tok][n_heads][head_dim] rotated to pos (a ``Rope``; inverse turns back)."""
+        self._ok(self.lib.aspida_rope_dev(rope.h, type, x, x_stride, n_tok, n_heads, head_dim, pos,
+                                          1 if inverse else 0, y, y_stride, stream), "aspida_rope_dev")
+
+    def kv4_page_bytes(self, head_dim, n_kv):
+        return int(self.lib.aspida_kv4_page_bytes(head_dim, n_kv))
+
+    def kv4_append(self, cache, type, k, k_stride, v, v_stride, n_rows, n_seq, row_start, kv_len, rope=None, pos=0,
+                   stream=0):
+        """Write key and value rows into a ``KV4Cache``, keys rotated to pos by rope (None: as they are)."""
+        self._ok(self.lib.aspida_kv4_append_dev(cache.ref, type, k, k_stride, v, v_stride, n_rows, n_seq, row_start,
+                                                kv_len, rope.h if rope else None, pos, stream),
+                 "aspida_kv4_append_dev")
+
+    def kv4_read(self, cache, type, n_rows, n_seq, row_start, kv_len, k, k_stride, v, v_stride, stream=0):
+        self._ok(self.lib.aspida_kv4_read_dev(cache.ref, type, n_rows, n_seq, row_start, kv_len, k, k_stride, v,
+                                              v_stride, stream), "aspida_kv4_read_dev")
+
+    def kv4_attention_work_bytes(self, cache, n_heads, n_rows, n_seq, max_rows):
+        n = int(self.lib.aspida_kv4_attn_work_bytes(cache.ref, n_heads, n_rows, n_seq, max_rows))
+        if n < 0:
+            raise ValueError(f"aspida_kv4_attn_work_bytes: bad arguments ({n_heads}, {n_rows}, {n_seq}, {max_rows})")
+        return n
+
+    def kv4_attention(self, cache, type, q, q_stride, n_heads, n_rows, n_seq, row_start, max_rows, kv_len, scale, out,
+                      out_stride, work, stream=0, window=0, lse=0):
+        """Attention of q's rows over the cache; lse receives log-sum-exps when given."""
+        self._ok(self.lib.aspida_kv4_attn_dev(cache.ref, type, q, q_stride, n_heads, n_rows, n_seq, row_start,
+                                              max_rows, kv_len, scale, window, out, out_stride, lse, work, stream),
+                 "aspida_kv4_attn_dev")
+
+    def kv4_weigh(self, cache, type, q, q_stride, n_heads, n_rows, n_seq, row_start, max_rows, kv_len, scale, lse,
+                  acc_in, acc_out, acc_stride, stream=0, window=0):
+        """acc_out = acc_in (0: zeros) + the attention weight each slot receives from q's rows."""
+        self._ok(self.lib.aspida_kv4_weigh_dev(cache.ref, type, q, q_stride, n_heads, n_rows, n_seq, row_start,
+                                               max_rows, kv_len, scale, window, lse, acc_in, acc_out, acc_stride,
+                                               stream), "aspida_kv4_weigh_dev")
+
+    def kv4_evict(self, src, n_seq, kv_len, acc, acc_stride, keep, first, recent, dst, new_len, idx, acc_out,
+                  stream=0):
+        """Keep the heaviest `keep` slots of each sequence and kv head, in order, in dst's pages."""
+        self._ok(self.lib.aspida_kv4_evict_dev(src.ref, n_seq, kv_len, acc, acc_stride, keep, first, recent, dst.ref,
+                                               new_len, idx, acc_out, stream), "aspida_kv4_evict_dev")
+
     def chain(self, steps):
         """A resident decode chain over steps [(kind, packed_ptr, in_dim, out_dim, x_ptr, y_ptr), ...]."""
         return Chain(self.lib, steps)
@@ -378,6 +435,73 @@ class DeviceOps:
         """Batches > 1: 0 built-in choice, 1 VALU, 2 64-vector MFMA, 3 16-vector MFMA,
         4 one-pass MFMA, 5 batch-1 MFMA on up to 4 vectors, 6 wave-per-column MFMA."""
         self._ok(self.lib.aspida_kq_set_mm_engine(engine), "aspida_kq_set_mm_engine")
+
+
+# Activation types of the rotary and cache calls.
+F32, F16, BF16 = 0, 1, 2
+
+
+class _RopeParams(ctypes.Structure):
+    """aspida_rope_params (include/aspidagpu.h)."""
+    _fields_ = [("rot_dim", ctypes.c_int), ("interleaved", ctypes.c_int), ("scaling", ctypes.c_int),
+                ("reserved", ctypes.c_int)] + [(n, ctypes.c_double) for n in ("base", "factor", "low", "high",
+                                                                              "context", "magnitude")] + \
+               [("freq_factors", ctypes.c_void_p)]
+
+
+class Rope:
+    """A rotation (aspida_rope_create): layout "half" or "interleaved", scaling
+    "none", "linear", "bands" or "yarn" (include/aspidagpu.h says what each
+    takes), freq_factors an array of rot_dim / 2 or None."""
+    SCALINGS = ("none", "linear", "bands", "yarn")
+
+    def __init__(self, rot_dim, base=10000.0, layout="half", scaling="none", factor=1.0, low=1.0, high=4.0,
+                 context=0, magnitude=0.0, freq_factors=None, path=None):
+        self.h = None
+        if layout not in ("half", "interleaved") or scaling not in self.SCALINGS:
+            raise ValueError(f"Rope: layout {layout!r}, scaling {scaling!r}")
+        ff = None if freq_factors is None else np.ascontiguousarray(freq_factors, np.float32)
+        if ff is not None and ff.size != rot_dim // 2:
+            raise ValueError(f"Rope: {ff.size} freq_factors for {rot_dim // 2} pairs")
+        self.lib, self.rot_dim = load(path), rot_dim
+        p = _RopeParams(rot_dim, int(layout == "interleaved"), self.SCALINGS.index(scaling), 0, base, factor, low,
+                        high, context, magnitude, None if ff is None else ff.ctypes.data)
+        self.h = self.lib.aspida_rope_create(ctypes.byref(p))
+        if not self.h:
+            raise RuntimeError(f"aspida_rope_create failed (error {self.lib.aspida_gpu_last_error()})")
+
+    def table(self):
+        """(angle per position of each pair, multiplier)."""
+        f, m = np.empty(self.rot_dim // 2), ctypes.c_double()
+        self.lib.aspida_rope_table(self.h, _p(f), ctypes.byref(m))
+        return f, m.value
+
+    def close(self):
+        if self.h:
+            self.lib.aspida_rope_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class _Kv4(ctypes.Structure):
+    """aspida_kv4 (include/aspidagpu.h)."""
+    _fields_ = [("head_dim", ctypes.c_int), ("n_kv", ctypes.c_int), ("n_pages", ctypes.c_int),
+                ("max_pages", ctypes.c_int), ("pages", ctypes.c_void_p), ("table", ctypes.c_void_p)]
+
+
+class KV4Cache:
+    """One layer's 4-bit key/value cache: device addresses of its pages
+    (n_pages * ``DeviceOps.kv4_page_bytes``) and page table [n_seq][max_pages]."""
+    PAGE = 64
+
+    def __init__(self, head_dim, n_kv, n_pages, max_pages, pages, table):
+        self.c = _Kv4(head_dim, n_kv, n_pages, max_pages, pages, table)
+        self.ref = ctypes.byref(self.c)
 
 
 class KqStep(ctypes.Structure):

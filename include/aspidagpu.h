@@ -228,6 +228,126 @@ int aspida_moe_experts_packed_dev(const float *x, int T, int dim, int top_k, int
                                   const void *shg_p, const void *shu_p, const void *shd_p,
                                   const float *shared_gate_inp, void *work, float *y, void *stream);
 
+/* ---- rotary positions and the 4-bit key/value cache ---------------------------
+ * What a decoder layer does between its q|k|v and its output product, on
+ * device pointers.  No counterpart in the reference ABI, whose attention lives
+ * behind its resident chain (gpu/gpu_matvec.cu:2063-2141).
+ * Activation types: 0 = f32, 1 = f16, 2 = bf16; operands need the alignment
+ * of their type only, and rows lie `stride` elements apart (at least heads *
+ * head_dim, which are contiguous).  Sums, softmax statistics and lse are f32.
+ * The calls allocate nothing, keep nothing and may be captured into a graph
+ * (its replays read the device arrays anew: lengths, row starts, tables). */
+
+/* A rotation: pair i of a head's first rot_dim values (even, 2 to 256) turns
+ * by pos * f_i, f_i = base^(-2 i / rot_dim); the angle is formed in f64.
+ * Pairs are (i, i + rot_dim / 2), or (2 i, 2 i + 1) when interleaved; the
+ * values behind rot_dim pass through.  freq_factors (host, rot_dim / 2 values
+ * as in a GGUF rope_freqs.weight, or NULL) divide f first.  scaling:
+ *   0 none;
+ *   1 linear: f / factor;
+ *   2 bands: f / factor for pairs that turn fewer than `low` times over
+ *     `context` positions, f for those that turn more than `high` times, and
+ *     a blend linear in the turns between;
+ *   3 blend by pair (YaRN): f / factor from the pair that turns `low` times on,
+ *     f up to the one that turns `high` times, linear in the pair between;
+ *     the rotated values are also multiplied by 0.1 ln(factor) + 1.
+ * magnitude, when not 0, replaces that multiplier (1 for the other scalings).
+ * aspida_rope_create returns a handle (host memory only; NULL and
+ * aspida_gpu_last_error on bad parameters); aspida_rope_table copies its
+ * rot_dim / 2 frequencies and multiplier out. */
+typedef struct aspida_rope_params {
+  int rot_dim, interleaved, scaling, reserved;
+  double base, factor, low, high, context, magnitude;
+  const float *freq_factors;
+} aspida_rope_params;
+void *aspida_rope_create(const aspida_rope_params *params);
+int aspida_rope_table(const void *rope, double *freq, double *magnitude);
+void aspida_rope_destroy(void *rope);
+
+/* y = x [n_tok][n_heads][head_dim] with every head rotated to its token's
+ * pos[n_tok] (any int); y may be x with the same stride, else they must not
+ * overlap.  inverse != 0 turns back: with magnitude 1 that undoes the
+ * rotation, and in general it is the gradient (y = dL/dx of x = dL/dy).
+ * -ENOTSUP for heads of more than 256 of the widest pieces (16 bytes, two
+ * values, one) that divide their runs. */
+int aspida_rope_dev(const void *rope, int type, const void *x, long long x_stride, int n_tok, int n_heads,
+                    int head_dim, const int *pos, int inverse, void *y, long long y_stride, void *stream);
+
+/* The cache of one layer: pages of 64 slots, each aspida_kv4_page_bytes long
+ * (80 head_dim per kv head: 5 bits a value), and per sequence a row of
+ * max_pages page ids; slot j of sequence b is in page table[b][j / 64].  A
+ * sequence's token t is at slot t, until an eviction.  head_dim is 64, 128 or
+ * 256.  Every 32 values x of a token's head keep m = f16(min x), a step d
+ * ((max x - m) / 15 rounded up to 7 significant bits, f16) and 4-bit codes q,
+ * the integers nearest (x - m) / d (ties to even): a code stands for
+ * d q + m.  A group with a value that is not finite, a minimum beyond f16 or
+ * a step above 254 reads back as NaN.
+ * Page ids outside [0, n_pages) and slots past max_pages name no memory:
+ * appends to them are dropped, reads give NaN, and a row that sees such a slot
+ * comes out as NaN.  No two table entries that a call writes to may name the
+ * same page.  pages is 16-byte aligned. */
+typedef struct aspida_kv4 {
+  int head_dim, n_kv, n_pages, max_pages;
+  void *pages;       /* device, n_pages * aspida_kv4_page_bytes(head_dim, n_kv) */
+  const int *table;  /* device, [n_seq][max_pages] */
+} aspida_kv4;
+long long aspida_kv4_page_bytes(int head_dim, int n_kv);
+
+/* Rows of new tokens, in the calls below: sequence b has rows row_start[b] ..
+ * row_start[b + 1] - 1 (device, n_seq + 1 ascending values up to n_rows; NULL:
+ * one row each, n_rows = n_seq).  kv_len[b] (device) is its length with them:
+ * its n rows are the tokens at slots kv_len[b] - n .. kv_len[b] - 1, those
+ * below 0 being left out.  Rows past the last sequence are not touched.  At
+ * most 65535 sequences; 0 rows or sequences are a no-op. */
+
+/* Writes k and v rows [n_rows][n_kv][head_dim] into the cache.  With a rope
+ * (rot_dim <= head_dim) keys are rotated to pos[n_rows] first, in f64 and
+ * rounded to f32 once; NULL stores them as they are. */
+int aspida_kv4_append_dev(const aspida_kv4 *cache, int type, const void *k, long long k_stride, const void *v,
+                          long long v_stride, int n_rows, int n_seq, const int *row_start, const int *kv_len,
+                          const void *rope, const int *pos, void *stream);
+
+/* The values the cache stands for, at the slots of such rows. */
+int aspida_kv4_read_dev(const aspida_kv4 *cache, int type, int n_rows, int n_seq, const int *row_start,
+                        const int *kv_len, void *k, long long k_stride, void *v, long long v_stride, void *stream);
+
+/* out[row][h] = sum_j softmax_j(scale * q[row][h] . k_j) v_j for q rows
+ * [n_rows][n_heads][head_dim] that are already in the cache: the row at slot
+ * p sees slots j <= p, and with window > 0 only j > p - window.  Query heads
+ * h * n_kv / n_heads share kv heads (n_heads a multiple of n_kv).  lse (NULL
+ * or [n_rows][n_heads]) receives log sum_j exp(scale * q . k_j).  A row that
+ * sees nothing (kv_len 0, or a slot below 0) gets 0, and lse -inf; what masked
+ * slots hold never matters.  max_rows: the rows of the longest sequence
+ * (larger or smaller values cost time, not correctness).  work: 256-byte
+ * aligned, aspida_kv4_attn_work_bytes for the same arguments; launches that
+ * share it must be ordered.  out must not overlap q. */
+long long aspida_kv4_attn_work_bytes(const aspida_kv4 *cache, int n_heads, int n_rows, int n_seq, int max_rows);
+int aspida_kv4_attn_dev(const aspida_kv4 *cache, int type, const void *q, long long q_stride, int n_heads, int n_rows,
+                        int n_seq, const int *row_start, int max_rows, const int *kv_len, float scale, int window,
+                        void *out, long long out_stride, float *lse, void *work, void *stream);
+
+/* The attention weight that each slot receives from such rows, given their
+ * lse: acc_out[b][g][j] = acc_in[b][g][j] + the sum over b's rows that see j
+ * and the query heads of kv head g of exp(scale * q . k_j - lse), nothing for
+ * slots from kv_len[b] on; both [n_seq][n_kv][acc_stride], slots past
+ * acc_stride being left out.  acc_in may be acc_out, or NULL for zeros.  The
+ * same bits every time (no atomics). */
+int aspida_kv4_weigh_dev(const aspida_kv4 *cache, int type, const void *q, long long q_stride, int n_heads, int n_rows,
+                         int n_seq, const int *row_start, int max_rows, const int *kv_len, float scale, int window,
+                         const float *lse, const float *acc_in, float *acc_out, long long acc_stride, void *stream);
+
+/* Shrinks each sequence to `keep` slots, per kv head: of kv_len[b] > keep
+ * slots the first `first` and the last `recent` stay, and of the others the
+ * heaviest by acc (NaN, negative and missing weights count as 0), among equals
+ * the lowest; they move in order to slots 0 .. keep - 1 of dst's pages (same
+ * head_dim and n_kv, its own table, no page in common with what src's table
+ * names).  Shorter sequences are copied.  new_len[n_seq] = min(kv_len, keep);
+ * idx and acc_out [n_seq][n_kv][keep] hold the old slot and weight of each
+ * new one, -1 and 0 past new_len.  first + recent <= keep. */
+int aspida_kv4_evict_dev(const aspida_kv4 *src, int n_seq, const int *kv_len, const float *acc, long long acc_stride,
+                         int keep, int first, int recent, const aspida_kv4 *dst, int *new_len, int *idx,
+                         float *acc_out, void *stream);
+
 /* Resident decode chain: an ordered list of packed matvecs (steps) run by ONE
  * persistent launch, with no launch boundary between them -- e.g. every
  * weight matrix of a decoder pass.  A step whose x lies inside an earlier
