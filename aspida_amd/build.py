@@ -32,7 +32,10 @@ CFLAGS = [
 # from the 64-row column loops (Q2_K / Q3_K / Q5_K launches of 28672x4096 and
 # up 2-7% faster, the 8B decode +0.2%); the small-batch sources measured equal
 # or slower with it (Q4_K 4096^2 at 64 vectors +12%), so only this file.
-EXTRA_FLAGS = {"kq_mv_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+# kv4_attn.hip: without it the decode attention's sums sit in AGPRs beside its
+# 192 VGPRs (228 in all, now 196).
+EXTRA_FLAGS = {"kq_mv_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+               "kv4_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _compile(src):

@@ -4,76 +4,364 @@
 // the slots j <= p (and j > p - window):
 //   o = sum_j softmax_j(scale q . k_j) v_j,   lse = log sum_j exp(scale q . k_j).
 // A row that sees nothing gets o = 0 and lse = -inf.
-#include "kv4.h"
+//
+// kv4_attn_split: the rows of a sequence times the query heads of a kv head
+// are columns, 16 to a tile.  A wave takes 32 tokens at a time:
+//   S[token][col] = K Q^T   16x16x32, K's codes as exact f16 (kv4_mma.h), one
+//                           more step for the minima; two planes of Q for f32
+//   P = exp2(S - ref)       ref follows the running maximum per column, moved
+//                           only when a score passes it by 2^8
+//   O[dim][col] += V^T P    P in S's own registers: S's lane holds tokens 4 rg
+//                           + 0..3 of two tiles for one column, which is how
+//                           the value dwords are ordered; one more step for
+//                           the minima
+// so nothing passes through LDS until the waves of a workgroup are joined.
+// A sequence's slots are cut into chunks of a length that all workgroups
+// derive from the lengths on the device (the host does not know them), so
+// that all chunks together fill the card; a second launch joins them.
+#include <algorithm>
+
+#include "kv4_mma.h"
 
 namespace kq {
 
-template <class T, int D>
-__global__ __launch_bounds__(256) void kv4_attn_simple(Kv4View c, Kv4Rows rows, Kv4Attn a) {
-  using L = Kv4L<D>;
-  __shared__ float q[D], s[64];
-  const int h = blockIdx.x, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
-  const Kv4Span sp = kv4_span(rows, b);
-  const int hk = h / (a.n_heads / c.n_kv);
-  for (int r = sp.r0 + blockIdx.y; r < sp.r1; r += gridDim.y) {
-    __syncthreads();
-    for (int i = tid; i < D; i += 256) q[i] = (float)((const T*)a.q)[(size_t)r * a.q_stride + (size_t)h * D + i] * a.scale;
-    for (int i = tid; i < D; i += 256) q[i] = __builtin_isfinite(q[i]) ? q[i] : __builtin_nanf("");
-    const int pos = sp.len - (sp.r1 - r);
-    const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    float m = -1e30f, l = 0.f, o = 0.f;
-    for (int p = lo / 64; p <= (pos >= 0 ? pos / 64 : -1); ++p) {
-      const uint8_t* blk = kv4_block(c, b, p, hk, L::BYTES);
-      __syncthreads();
-      const int t = tid >> 2, part = tid & 3;
-      float dot = 0.f;
-      for (int g = 0; g < L::NG; ++g) {
-        const uint32_t wd = blk ? *reinterpret_cast<const uint32_t*>(blk + L::key_word(t, g, part)) : 0;
-        const float d = blk ? kv4_f16(blk + L::key_d(t, g)) : __builtin_nanf(""), mm = blk ? kv4_f16(blk + L::key_m(t, g)) : 0.f;
-        for (int j = 0; j < 8; ++j) dot += q[32 * g + 8 * part + j] * __builtin_fmaf(d, (float)kv4_code(wd, j), mm);
-      }
-      dot += __shfl_xor(dot, 1, 64);
-      dot += __shfl_xor(dot, 2, 64);
-      if (part == 0) s[t] = (p * 64 + t <= pos && p * 64 + t >= lo) ? dot : -INFINITY;
-      __syncthreads();
-      float mx = s[lane];
-      for (int k = 32; k; k >>= 1) mx = fmaxf(mx, __shfl_xor(mx, k, 64));
-      const float mn = fmaxf(m, mx), f = expf(m - mn);
-      float pr = expf(s[lane] - mn), ps = pr;
-      for (int k = 32; k; k >>= 1) ps += __shfl_xor(ps, k, 64);
-      l = l * f + ps;
-      o *= f;
-      m = mn;
-      if (tid < D)
-        for (int t2 = 0; t2 < 64; ++t2) {
-          if (!(p * 64 + t2 <= pos && p * 64 + t2 >= lo)) continue;
-          const uint32_t wd = blk ? *reinterpret_cast<const uint32_t*>(blk + L::value_word(t2, tid)) : 0;
-          const float d = blk ? kv4_f16(blk + L::value_d(t2, tid >> 5)) : __builtin_nanf(""), mm = blk ? kv4_f16(blk + L::value_m(t2, tid >> 5)) : 0.f;
-          o += expf(s[t2] - mn) * __builtin_fmaf(d, (float)kv4_code(wd, L::value_j(t2)), mm);
-        }
+constexpr int ATTN_WAVES = 4;
+constexpr int ATTN_STEP = 32 * ATTN_WAVES;  // tokens of a workgroup's round
+// Workgroups that the chunks are cut for: three for each of 256 CUs.
+constexpr int ATTN_GROUPS = 768;
+constexpr float REF0 = -3.402823466e38f;  // below every score
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+
+// Slots that a sequence's rows see together: [lo, hi), lo a multiple of 32.
+struct SeenRange { int lo, hi; };
+__device__ __forceinline__ SeenRange seen_range(const Kv4Span& s, int window, int max_slots) {
+  const int first = s.len - (s.r1 - s.r0);  // the first row's slot
+  SeenRange r;
+  r.hi = s.r1 > s.r0 ? min(s.len, max_slots) : 0;
+  r.lo = window > 0 ? min(max(0, first - window + 1) & ~31, r.hi & ~31) : 0;
+  return r;
+}
+
+// How the sequences' slots are cut.  Every wave derives the same: chunk, the
+// tokens of a chunk, and for a workgroup number x its sequence and chunk
+// (seq < 0: none), with the sequence's chunks and the number of its first.
+struct Cut { int seq, index, count, first, chunk; };
+
+__device__ __forceinline__ int chunk_tokens(const Kv4Rows& rows, int window, int max_slots, int per_seq) {
+  const int lane = threadIdx.x & 63;
+  float total = 0.f;
+  for (int b = lane; b < rows.n_seq; b += 64) {
+    const SeenRange r = seen_range(kv4_span(rows, b), window, max_slots);
+    total += (float)max(r.hi - r.lo, 0);
+  }
+  total = wave_total(total) * (float)per_seq;
+  const float want = total / (float)ATTN_GROUPS;
+  const int steps = (int)fminf(ceilf(want / (float)ATTN_STEP), 8388608.f);
+  return max(1, steps) * ATTN_STEP;
+}
+
+__device__ __forceinline__ int chunks_of(const Kv4Rows& rows, int b, int window, int max_slots, int chunk) {
+  const SeenRange r = seen_range(kv4_span(rows, b), window, max_slots);
+  return max(1, (r.hi - r.lo + chunk - 1) / chunk);
+}
+
+__device__ __forceinline__ Cut cut_of(const Kv4Rows& rows, int window, int max_slots, int per_seq, int x) {
+  const int lane = threadIdx.x & 63;
+  Cut c;
+  c.chunk = chunk_tokens(rows, window, max_slots, per_seq);
+  int before = 0;
+  for (int b0 = 0; b0 < rows.n_seq; b0 += 64) {
+    const int n = b0 + lane < rows.n_seq ? chunks_of(rows, b0 + lane, window, max_slots, c.chunk) : 0;
+    const int end = before + wave_scan_add(n);
+    const uint64_t over = __ballot(end > x);
+    if (over) {
+      const int l = __builtin_ctzll(over);
+      c.seq = b0 + l;
+      c.count = __builtin_amdgcn_readlane(n, l);
+      c.first = __builtin_amdgcn_readlane(end, l) - c.count;
+      c.index = x - c.first;
+      return c;
     }
-    if (tid < D) ((T*)a.out)[(size_t)r * a.out_stride + (size_t)h * D + tid] = (T)(l != 0.f ? o / l : 0.f);
-    if (tid == 0 && a.lse) a.lse[(size_t)r * a.n_heads + h] = l != 0.f ? m + logf(l) : -INFINITY;
+    before = __builtin_amdgcn_readlane(end, 63);
+  }
+  c.seq = -1;
+  c.index = c.count = c.first = 0;
+  return c;
+}
+
+// Workspace: per chunk, kv head and column tile the columns' sums [16][D] and
+// (ref, l) [16].
+template <int D> struct AttnPart {
+  float o[16][D];
+  float ref[16], l[16];
+};
+
+struct SplitArgs {
+  Kv4View c;
+  Kv4Rows rows;
+  Kv4Attn a;
+  int group, tiles;  // query heads of a kv head, column tiles
+};
+
+template <class T>
+__device__ __forceinline__ void store4(T* p, const float (&x)[4]) {
+  struct { T v[4]; } r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.v[i] = (T)x[i];
+  __builtin_memcpy(p, &r, sizeof(r));
+}
+
+// Rows past max_rows have no workgroup: NaN, by all threads of one.
+template <class T>
+__device__ void fill_excess(const SplitArgs& s, const Kv4Span& sp, int hk, int d) {
+  const int w = s.group * d;
+  for (int row = sp.r0 + s.a.max_rows; row < sp.r1; ++row) {
+    T* out = (T*)s.a.out + (size_t)row * s.a.out_stride + (size_t)hk * w;
+    for (int i = threadIdx.x; i < w; i += blockDim.x) out[i] = (T)__builtin_nanf("");
+    if (s.a.lse)
+      for (int i = threadIdx.x; i < s.group; i += blockDim.x)
+        s.a.lse[(size_t)row * s.a.n_heads + hk * s.group + i] = __builtin_nanf("");
   }
 }
 
+template <int D, class T>
+__global__ __launch_bounds__(64 * ATTN_WAVES) void kv4_attn_split(SplitArgs s) {
+  using L = Kv4L<D>;
+  constexpr bool TWO = sizeof(T) == 4;
+  constexpr int NG = D / 32, NT = D / 16;
+  __shared__ float so[2][16][D];
+  __shared__ float sr[2][16], sl[2][16];
+  const int lane = threadIdx.x & 63, col = lane & 15, rg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Cut cut = cut_of(s.rows, s.a.window, s.c.max_pages * KV4_PAGE, s.c.n_kv * s.tiles, blockIdx.x);
+  if (cut.seq < 0) return;
+  const int b = cut.seq, hk = blockIdx.y / s.tiles, tile = blockIdx.y % s.tiles;
+  const Kv4Span sp = kv4_span(s.rows, b);
+  const int n = sp.r1 - sp.r0;
+  if (n > s.a.max_rows && cut.index == 0 && tile == 0) fill_excess<T>(s, sp, hk, D);
+  const int ncol = min(16, min(n, s.a.max_rows) * s.group - tile * 16);
+  if (ncol <= 0) return;
+  // This lane's column: its row, head, and the slots [clo, chi) it sees.
+  const int ci = tile * 16 + col, row = ci / s.group, head = hk * s.group + ci % s.group;
+  const bool valid = col < ncol;
+  const int pos = sp.len - n + row;
+  const int chi = valid ? max(pos + 1, 0) : 0, clo = s.a.window > 0 ? max(0, pos - s.a.window + 1) : 0;
+  Query<D, TWO> q;
+  q.load((const T*)s.a.q + (size_t)(sp.r0 + (valid ? row : 0)) * s.a.q_stride + (size_t)head * D, valid, lane);
+  const float unit = q.unit * (s.a.scale * LOG2E);
+
+  // The chunk's slots, and those of them that every column sees.
+  const SeenRange seen = seen_range(sp, s.a.window, s.c.max_pages * KV4_PAGE);
+  const int t0 = seen.lo + cut.index * cut.chunk, t1 = min(seen.hi, t0 + cut.chunk);
+  const int row_last = (tile * 16 + ncol - 1) / s.group, row_first = tile * 16 / s.group;
+  const int all_hi = sp.len - n + row_first + 1;                                       // below: seen by every column
+  const int all_lo = s.a.window > 0 ? max(0, sp.len - n + row_last - s.a.window + 1) : 0;
+  const int any_hi = min(t1, sp.len - n + row_last + 1);
+  const int any_lo = s.a.window > 0 ? max(0, sp.len - n + row_first - s.a.window + 1) : 0;
+
+  kvf4 o[NT], om = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < NT; ++i) o[i] = om;
+  // A row past the table sees its own slot there: NaN.
+  float ref = REF0, l = chi > s.c.max_pages * KV4_PAGE && cut.index == 0 && wave == 0 ? __builtin_nanf("") : 0.f;
+
+  int t = t0 + 32 * wave;
+  KeyTile<D> k[2];
+  ValueBlock<D> v;
+  bool there = false;
+  auto load = [&](int at) {
+    const uint8_t* blk = kv4_block(s.c, b, at >> 6, hk, L::BYTES);
+    there = blk != nullptr;
+    if (!blk) blk = s.c.pages;  // any page: what is read there is not used
+    const int half = (at >> 5) & 1;
+    k[0].load(blk, 2 * half, lane);
+    k[1].load(blk, 2 * half + 1, lane);
+    v.load(blk, half, lane);
+  };
+  if (t < any_hi) load(t);
+  for (; t < any_hi; t += ATTN_STEP) {
+    kvf4 c[2] = {q.scores(k[0]), q.scores(k[1])};
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = c[j >> 2][j & 3] * unit;
+    ValueBlock<D> vv = v;
+    const bool ok = there;
+    const int at = t;
+    if (t + ATTN_STEP < any_hi) load(t + ATTN_STEP);
+    if (!ok || at + 32 > all_hi || at < all_lo) {
+      // Slots that this column does not see get no weight; the steps and
+      // minima of slots that no column sees may be anything and become 0.
+      uint32_t keep = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int slot = at + 16 * (j >> 2) + 4 * rg + (j & 3);
+        const bool see = slot >= clo && slot < chi;
+        x[j] = see ? (ok ? x[j] : __builtin_nanf("")) : -INFINITY;
+        if (ok && slot < any_hi && slot >= any_lo) keep |= 1u << j;
+      }
+      vv.drop(keep);
+    }
+    float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    if (__ballot(top > ref + 15.f)) {
+      // P' = exp2(x - ref) is kept below 2^15; after a move the maximum of the
+      // column is at 2^7.
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float next = fmaxf(ref, top - 7.f);
+      const float f = __builtin_amdgcn_exp2f(ref - next);
+      ref = next;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) o[i] *= f;
+      om *= f;
+    }
+    kvh8 ph, pl;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float p = __builtin_amdgcn_exp2f(x[j] - ref);
+      l += p;
+      ph[j] = (_Float16)p;
+      if constexpr (TWO) pl[j] = (_Float16)(p - (float)ph[j]);
+    }
+    const kvh8 vm = __builtin_bit_cast(kvh8, vv.m);
+    if constexpr (TWO) om = kv_mfma(vm, pl, om);
+    om = kv_mfma(vm, ph, om);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const kvh2 d0 = kv_h2(vv.d[g][0]), d1 = kv_h2(vv.d[g][1]), d2 = kv_h2(vv.d[g][2]), d3 = kv_h2(vv.d[g][3]);
+      const kvh2 n0 = kv_times(d0, -16.f), n1 = kv_times(d1, -256.f), n2 = kv_times(d2, -16.f), n3 = kv_times(d3, -256.f);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = 2 * g + e;
+        const kvh8 a = kv4_unpack(vv.w[i >> 2][i & 3], d0, d1, d2, d3, n0, n1, n2, n3);
+        if constexpr (TWO) o[i] = kv_mfma(a, pl, o[i]);
+        o[i] = kv_mfma(a, ph, o[i]);
+      }
+    }
+  }
+
+  // The wave's column sums: l over the lane groups, and the minima's part of
+  // dim group g (row g of om) added to its dims.
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    const float part = __shfl(om[g & 3], (g >> 2) * 16 + col, 64);
+    o[2 * g] += part;
+    o[2 * g + 1] += part;
+  }
+  // Join the waves, pairs first: the upper of a pair hands over its sums.
+#pragma unroll
+  for (int half = ATTN_WAVES / 2; half >= 1; half >>= 1) {
+    __syncthreads();
+    if (wave >= half && wave < 2 * half) {
+      const int w = wave - half;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) *reinterpret_cast<kvf4*>(&so[w][col][16 * i + 4 * rg]) = o[i];
+      if (rg == 0) { sr[w][col] = ref; sl[w][col] = l; }
+    }
+    __syncthreads();
+    if (wave < half) {
+      const float r2 = sr[wave][col], next = fmaxf(ref, r2);
+      const float f = __builtin_amdgcn_exp2f(ref - next), f2 = __builtin_amdgcn_exp2f(r2 - next);
+      ref = next;
+      l = l * f + sl[wave][col] * f2;
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+        o[i] = o[i] * f + *reinterpret_cast<const kvf4*>(&so[wave][col][16 * i + 4 * rg]) * f2;
+    }
+  }
+  if (wave != 0 || !valid) return;
+  if (cut.count == 1) {
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    T* out = (T*)s.a.out + (size_t)(sp.r0 + row) * s.a.out_stride + (size_t)head * D;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const float y[4] = {o[i][0] * inv, o[i][1] * inv, o[i][2] * inv, o[i][3] * inv};
+      store4(out + 16 * i + 4 * rg, y);
+    }
+    if (s.a.lse && rg == 0)
+      s.a.lse[(size_t)(sp.r0 + row) * s.a.n_heads + head] = l != 0.f ? (ref + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+    return;
+  }
+  AttnPart<D>* part = (AttnPart<D>*)s.a.work + (size_t)blockIdx.x * gridDim.y + blockIdx.y;
+#pragma unroll
+  for (int i = 0; i < NT; ++i) *reinterpret_cast<kvf4*>(&part->o[col][16 * i + 4 * rg]) = o[i];
+  if (rg == 0) { part->ref[col] = ref; part->l[col] = l; }
+}
+
+// Joins the chunks of a sequence: a workgroup per (kv head and column tile,
+// sequence), a wave per column in turn.
+template <int D, class T>
+__global__ __launch_bounds__(256) void kv4_attn_join(SplitArgs s) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int b = blockIdx.y, hk = blockIdx.x / s.tiles, tile = blockIdx.x % s.tiles;
+  const Kv4Span sp = kv4_span(s.rows, b);
+  const int ncol = min(16, min(sp.r1 - sp.r0, s.a.max_rows) * s.group - tile * 16);
+  if (ncol <= 0) return;
+  const int slots = s.c.max_pages * KV4_PAGE;
+  const int chunk = chunk_tokens(s.rows, s.a.window, slots, s.c.n_kv * s.tiles);
+  const int count = chunks_of(s.rows, b, s.a.window, slots, chunk);
+  if (count == 1) return;
+  int first = 0;
+  for (int i = lane; i < b; i += 64) first += chunks_of(s.rows, i, s.a.window, slots, chunk);
+  for (int o = 32; o; o >>= 1) first += __shfl_xor(first, o, 64);
+  const AttnPart<D>* part = (const AttnPart<D>*)s.a.work + (size_t)first * gridDim.x + blockIdx.x;
+  const size_t step = gridDim.x;
+  for (int col = wave; col < ncol; col += 4) {
+    float ref = REF0;
+    for (int i = lane; i < count; i += 64) ref = fmaxf(ref, part[i * step].ref[col]);
+    for (int o = 32; o; o >>= 1) ref = fmaxf(ref, __shfl_xor(ref, o, 64));
+    float l = 0.f, y[D / 64] = {};
+    for (int i = 0; i < count; ++i) {
+      const AttnPart<D>& p = part[i * step];
+      const float f = __builtin_amdgcn_exp2f(p.ref[col] - ref);
+      l += p.l[col] * f;
+#pragma unroll
+      for (int e = 0; e < D / 64; ++e) y[e] += p.o[col][lane + 64 * e] * f;
+    }
+    const int ci = tile * 16 + col, row = sp.r0 + ci / s.group, head = hk * s.group + ci % s.group;
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e)
+      ((T*)s.a.out)[(size_t)row * s.a.out_stride + (size_t)head * D + lane + 64 * e] = (T)(y[e] * inv);
+    if (s.a.lse && lane == 0)
+      s.a.lse[(size_t)row * s.a.n_heads + head] = l != 0.f ? (ref + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+  }
+}
+
+static int attn_tiles(int group, int max_rows) { return (int)std::min<long long>(65535, ((long long)max_rows * group + 15) / 16); }
+// Chunks of all sequences: their total over the chunk length, which is at
+// least total * per_seq / ATTN_GROUPS, and one more for each sequence.
+static int attn_chunks(int per_seq, int n_seq) { return (ATTN_GROUPS + per_seq - 1) / per_seq + n_seq; }
+
 size_t kv4_attn_work_bytes(int head_dim, int n_kv, int n_heads, int n_rows, int n_seq, int max_rows, int max_pages) {
-  return 256;
+  const int tiles = attn_tiles(n_heads / n_kv, max_rows), per_seq = n_kv * tiles;
+  const size_t part = 16 * (size_t)head_dim * 4 + 128;
+  return std::max<size_t>(256, (size_t)attn_chunks(per_seq, n_seq) * per_seq * part);
+}
+
+template <int D, class T>
+static void attn_go(const SplitArgs& s, hipStream_t st) {
+  const int per_seq = s.c.n_kv * s.tiles;
+  hipLaunchKernelGGL((kv4_attn_split<D, T>), dim3(attn_chunks(per_seq, s.rows.n_seq), per_seq), dim3(64 * ATTN_WAVES), 0, st, s);
+  hipLaunchKernelGGL((kv4_attn_join<D, T>), dim3(per_seq, s.rows.n_seq), dim3(256), 0, st, s);
 }
 
 template <class T>
-static void attn_typed(int head_dim, const Kv4View& c, const Kv4Rows& rows, const Kv4Attn& a, hipStream_t s) {
-  const dim3 grid(a.n_heads, a.max_rows < 4096 ? a.max_rows : 4096, rows.n_seq);
-  if (head_dim == 64) hipLaunchKernelGGL((kv4_attn_simple<T, 64>), grid, dim3(256), 0, s, c, rows, a);
-  else if (head_dim == 128) hipLaunchKernelGGL((kv4_attn_simple<T, 128>), grid, dim3(256), 0, s, c, rows, a);
-  else hipLaunchKernelGGL((kv4_attn_simple<T, 256>), grid, dim3(256), 0, s, c, rows, a);
+static void attn_typed(int head_dim, const SplitArgs& s, hipStream_t st) {
+  if (head_dim == 64) attn_go<64, T>(s, st);
+  else if (head_dim == 128) attn_go<128, T>(s, st);
+  else attn_go<256, T>(s, st);
 }
 
 hipError_t launch_kv4_attn(int head_dim, const Kv4View& c, int type, const Kv4Rows& rows, const Kv4Attn& a,
-                           hipStream_t s) {
-  if (type == ACT_F32) attn_typed<float>(head_dim, c, rows, a, s);
-  else if (type == ACT_F16) attn_typed<_Float16>(head_dim, c, rows, a, s);
-  else attn_typed<bf16_t>(head_dim, c, rows, a, s);
+                           hipStream_t st) {
+  SplitArgs s{c, rows, a, a.n_heads / c.n_kv, attn_tiles(a.n_heads / c.n_kv, a.max_rows)};
+  if (type == ACT_F32) attn_typed<float>(head_dim, s, st);
+  else if (type == ACT_F16) attn_typed<_Float16>(head_dim, s, st);
+  else attn_typed<bf16_t>(head_dim, s, st);
   return hipGetLastError();
 }
 

@@ -5,7 +5,10 @@
 //   d = r rounded up to 7 significant bits (a multiple of 2^-24 at least),
 //   q = the nearest integer to (x - m) / d, ties to even, within 0 .. 15,
 // d = 0 and q = 0 where r <= 0.  A group with a value that is not finite, or
-// a minimum or step beyond the format, gets d = NaN and reads back as NaN.
+// a minimum or step beyond the format, has d = m = 0, and its token's key in
+// that head gets d = NaN in every group: key and value read back as NaN, and
+// scores of the slot are NaN, while value scales are always finite (a weight
+// of 0 times them is 0).
 // The arithmetic is exact (f64 differences, remainders by fma): a code never
 // depends on how a quotient was rounded.
 #include <algorithm>
@@ -23,7 +26,7 @@ struct AppendArgs {
   RopeTable t;
 };
 
-struct Kv4Group { float d, m; int q[4]; };
+struct Kv4Group { float d, m; int q[4]; bool bad; };
 
 // Quantises a group from four values in each of eight neighbouring lanes.
 __device__ __forceinline__ Kv4Group kv4_quantise(const float (&x)[4]) {
@@ -48,11 +51,12 @@ __device__ __forceinline__ Kv4Group kv4_quantise(const float (&x)[4]) {
     d = ldexp(ceil(ldexp(r, -step)), step);
   }
   if (bad || !__builtin_isfinite(g.m) || d > (double)KV4_D_MAX) {
-    g.d = __builtin_nanf("");
-    g.m = 0.f;
+    g.bad = true;
+    g.d = g.m = 0.f;
     g.q[0] = g.q[1] = g.q[2] = g.q[3] = 0;
     return g;
   }
+  g.bad = false;
   g.d = (float)d;
   const double inv = d > 0.0 ? 1.0 / d : 0.0;
 #pragma unroll
@@ -87,6 +91,7 @@ __global__ __launch_bounds__(256) void kv4_append(AppendArgs a) {
   using L = Kv4L<D>;
   __shared__ double2 cs[ROPE ? 16 * D / 2 : 1];  // cos, sin [token of the tile][pair]
   __shared__ uint8_t vq[32][D];
+  __shared__ int bad[32];  // the token's key or value holds a group that the format does not
   const int hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   const Kv4Span sp = kv4_span(a.rows, b);
   const int n = sp.r1 - sp.r0, slot0 = sp.len - n;  // the first row's slot, below 0 where kv_len < n
@@ -98,6 +103,24 @@ __global__ __launch_bounds__(256) void kv4_append(AppendArgs a) {
     if (!base) continue;
     const int s0 = blk << 5, p0 = (blk & 1) * 32;  // first slot, and its token of the page
     const int c8 = tid & 7;
+    if (tid < 32) bad[tid] = 0;
+    __syncthreads();
+#pragma unroll 2
+    for (int it = 0; it < L::NG; ++it) {
+      const int t = tid >> 3, g = it, slot = s0 + t;
+      const bool in = slot >= lo && slot < hi;
+      float x[4] = {0.f, 0.f, 0.f, 0.f};
+      if (in) load4((const T*)a.v + (size_t)(sp.r0 + (slot - slot0)) * a.vs + (size_t)hk * D + 32 * g + 4 * c8, x);
+      const Kv4Group q = kv4_quantise(x);
+      *reinterpret_cast<uint32_t*>(&vq[t][32 * g + 4 * c8]) =
+          (uint32_t)q.q[0] | (uint32_t)q.q[1] << 8 | (uint32_t)q.q[2] << 16 | (uint32_t)q.q[3] << 24;
+      if (in && c8 == 0) {
+        if (q.bad) bad[t] = 1;
+        *reinterpret_cast<_Float16*>(base + L::value_d(p0 + t, g)) = (_Float16)q.d;
+        *reinterpret_cast<_Float16*>(base + L::value_m(p0 + t, g)) = (_Float16)q.m;
+      }
+    }
+    __syncthreads();
     for (int tile = 0; tile < 2; ++tile) {
       const int f = s0 + 16 * tile;
       if (f >= hi || f + 16 <= lo) continue;
@@ -153,26 +176,12 @@ __global__ __launch_bounds__(256) void kv4_append(AppendArgs a) {
         const int tok = p0 + 16 * tile + t;
         if (in && !(c8 & 1)) *reinterpret_cast<uint32_t*>(base + L::key_word(tok, g, c8 >> 1)) = w;
         if (in && c8 == 0) {
+          if (q.bad) bad[16 * tile + t] = 1;
           *reinterpret_cast<_Float16*>(base + L::key_d(tok, g)) = (_Float16)q.d;
           *reinterpret_cast<_Float16*>(base + L::key_m(tok, g)) = (_Float16)q.m;
         }
       }
     }
-#pragma unroll 2
-    for (int it = 0; it < L::NG; ++it) {
-      const int t = tid >> 3, g = it, slot = s0 + t;
-      const bool in = slot >= lo && slot < hi;
-      float x[4] = {0.f, 0.f, 0.f, 0.f};
-      if (in) load4((const T*)a.v + (size_t)(sp.r0 + (slot - slot0)) * a.vs + (size_t)hk * D + 32 * g + 4 * c8, x);
-      const Kv4Group q = kv4_quantise(x);
-      *reinterpret_cast<uint32_t*>(&vq[t][32 * g + 4 * c8]) =
-          (uint32_t)q.q[0] | (uint32_t)q.q[1] << 8 | (uint32_t)q.q[2] << 16 | (uint32_t)q.q[3] << 24;
-      if (in && c8 == 0) {
-        *reinterpret_cast<_Float16*>(base + L::value_d(p0 + t, g)) = (_Float16)q.d;
-        *reinterpret_cast<_Float16*>(base + L::value_m(p0 + t, g)) = (_Float16)q.m;
-      }
-    }
-    __syncthreads();
     const bool whole = s0 >= lo && s0 + 32 <= hi;
     for (int i = tid; i < 4 * D; i += 256) {
       const int rg = i / D, d = i - rg * D;
@@ -189,6 +198,12 @@ __global__ __launch_bounds__(256) void kv4_append(AppendArgs a) {
       uint32_t* p = reinterpret_cast<uint32_t*>(base + L::value_word(p0 + 4 * rg, d));
       if (whole) *p = w;
       else if (mine) *p = (*p & ~mine) | w;
+    }
+    __syncthreads();
+    // (A slot that is not this call's has no flag.)
+    if (tid < 32 && bad[tid]) {
+#pragma unroll
+      for (int g = 0; g < L::NG; ++g) *reinterpret_cast<uint16_t*>(base + L::key_d(p0 + tid, g)) = 0x7E00;
     }
     __syncthreads();
   }
@@ -238,7 +253,7 @@ __global__ __launch_bounds__(256) void kv4_read(ReadArgs a) {
         const int t = 16 * (j >> 2) + 4 * rg + (j & 3), slot = s0 + t;
         if (slot >= lo && slot < hi) {
           float dd = __builtin_nanf(""), m = 0.f;
-          if (base) {
+          if (base && kv4_f16(base + L::key_d(p0 + t, 0)) >= 0.f) {
             dd = kv4_f16(base + L::value_d(p0 + t, d >> 5));
             m = kv4_f16(base + L::value_m(p0 + t, d >> 5));
           }

@@ -280,8 +280,9 @@ int aspida_rope_dev(const void *rope, int type, const void *x, long long x_strid
  * 256.  Every 32 values x of a token's head keep m = f16(min x), a step d
  * ((max x - m) / 15 rounded up to 7 significant bits, f16) and 4-bit codes q,
  * the integers nearest (x - m) / d (ties to even): a code stands for
- * d q + m.  A group with a value that is not finite, a minimum beyond f16 or
- * a step above 254 reads back as NaN.
+ * d q + m.  A token whose key or value in some kv head has a group with a
+ * value that is not finite, a minimum beyond f16 or a step above 254 reads
+ * back as NaN there, key and value, and a row that sees it comes out as NaN.
  * Page ids outside [0, n_pages) and slots past max_pages name no memory:
  * appends to them are dropped, reads give NaN, and a row that sees such a slot
  * comes out as NaN.  No two table entries that a call writes to may name the
@@ -317,8 +318,8 @@ int aspida_kv4_read_dev(const aspida_kv4 *cache, int type, int n_rows, int n_seq
  * h * n_kv / n_heads share kv heads (n_heads a multiple of n_kv).  lse (NULL
  * or [n_rows][n_heads]) receives log sum_j exp(scale * q . k_j).  A row that
  * sees nothing (kv_len 0, or a slot below 0) gets 0, and lse -inf; what masked
- * slots hold never matters.  max_rows: the rows of the longest sequence
- * (larger or smaller values cost time, not correctness).  work: 256-byte
+ * slots hold never matters.  max_rows: at least the rows of the longest
+ * sequence (what a sequence has past it comes out as NaN).  work: 256-byte
  * aligned, aspida_kv4_attn_work_bytes for the same arguments; launches that
  * share it must be ordered.  out must not overlap q. */
 long long aspida_kv4_attn_work_bytes(const aspida_kv4 *cache, int n_heads, int n_rows, int n_seq, int max_rows);

@@ -59,6 +59,15 @@ def stands_for(x):
     return (q * d[..., None] + m[..., None]).reshape(np.shape(x))
 
 
+def pair_stands_for(k, v):
+    """The same for the keys and values of the same tokens and heads: where
+    either has a group beyond the format, both are NaN."""
+    k, v = stands_for(k), stands_for(v)
+    bad = np.isnan(k).any(-1) | np.isnan(v).any(-1)
+    k[bad] = v[bad] = np.nan
+    return k, v
+
+
 def visible(n, rows, window):
     """bool [rows][n]: which slots each of the last `rows` of n tokens sees."""
     pos = np.arange(n - rows, n)[:, None]
@@ -69,20 +78,29 @@ def visible(n, rows, window):
     return see
 
 
+def parts(x):
+    """|d q| + |m| at least, of cached values x [..., dim]: a value is the sum
+    of its code's part and its group's minimum (code 0 occurs in each group)."""
+    m = x.reshape(*x.shape[:-1], -1, 32).min(-1)
+    return np.abs(x) + 2 * np.repeat(np.abs(m), 32, -1)
+
+
 def attend(q, k, v, scale, window=0):
-    """q [rows][heads][dim], k and v [n][kv][dim] f64 -> (out, lse, sum p |v|,
-    largest visible scale * sum |q k|) of the rows at the end of the n slots."""
+    """q [rows][heads][dim], k and v [n][kv][dim] f64 -> (out, lse, sum p parts(v),
+    largest visible scale * sum |q| parts(k)) of the rows at the end of the n
+    slots."""
     rows, heads, dim = q.shape
     n, kv, _ = k.shape
     out = np.zeros((rows, heads, dim))
     lse = np.full((rows, heads), -np.inf)
     pv, sk = np.zeros((rows, heads, dim)), np.zeros((rows, heads))
     see = visible(n, rows, window)
+    kp, vp = parts(k), parts(v)
     for h in range(heads):
         g = h * kv // heads
         with np.errstate(invalid="ignore"):
             s = q[:, h] @ k[:, g].T * scale
-            size = np.abs(q[:, h]) @ np.abs(k[:, g]).T * abs(scale)
+            size = np.abs(q[:, h]) @ kp[:, g].T * abs(scale)
         for r in range(rows):
             w = see[r]
             if not w.any():
@@ -92,7 +110,7 @@ def attend(q, k, v, scale, window=0):
             lse[r, h] = top + np.log(p.sum())
             p /= p.sum()
             out[r, h] = p @ v[w, g]
-            pv[r, h] = p @ np.abs(v[w, g])
+            pv[r, h] = p @ vp[w, g]
             sk[r, h] = size[r, w].max()
     return out, lse, pv, sk
 

@@ -7,12 +7,13 @@ Bounds, with u = 2^-24 (half a step of f32) and h_T half a step of the type:
   * append and read: the stored value exactly, rounded to f32 and the type;
   * scores: the two f16 planes of a query leave 2^-22 of each product, and the
     f32 sums at most 16 roundings of partial sums: S = 2^-19 of
-    scale sum |q k|;
+    scale sum |q| (|d code| + |m|), a key being summed as its code's part and
+    its minimum apart;
   * attention: a softmax weight is off by the two scores' errors, 2 S, exp
     (2^-22) and its own planes (2^-22), the sums by a rounding per addition
     of a lane (n / 16 + 64 of them at most): E_w = 2 S + 2^-20 +
     (n / 16 + 64) u.  With f16 and bf16 activations weights and values are
-    single f16 numbers: 2^-11 more each.  The output: E_w sum p |v|, plus h_T;
+    single f16 numbers: 2^-11 more each.  The output: E_w sum p (|d code| + |m|), plus h_T;
   * lse: S + 2^-20 + (n / 16 + 64) u + u |lse|;
   * weights of slots: each term S + u |score - lse| scale + 2^-20, all
     positive: summed.
@@ -219,7 +220,7 @@ def test_append_and_read(case, ty):
             c.append(ty, dk, dv, st, lens, rope, pos)
         else:
             c.append(ty, dk, dv, st, lens)
-        ks, vs = plain.stands_for(hk.astype(np.float32)), plain.stands_for(hv.astype(np.float32))
+        ks, vs = plain.pair_stands_for(hk.astype(np.float32), hv.astype(np.float32))
         for b in range(n_seq):
             want[b][0].append(ks[st[b]:st[b + 1]])
             want[b][1].append(vs[st[b]:st[b + 1]])
@@ -277,12 +278,14 @@ def test_append_of_ties_constants_and_values_beyond_the_format():
     x[6, 0, 3] = 4000.0                                   # a step above 254
     x[7, 0] = -0.0
     x[8, 0] = np.float32(1 + 2.0 ** -11) * (1 + np.arange(64) % 2)   # the f16 minimum lies above or below
-    c = Cache(gen, 64, 1, 1, 1)
-    c.append(aa.F32, _dev(x), _dev(x), [0, 9], [9])
-    k, v = c.read(aa.F32, [0, 9], [9])
-    want = plain.stands_for(x).astype(np.float32).astype(np.float64)
-    assert np.isnan(want[3:7]).reshape(4, 2, 32).any(-1).sum() == 4
-    assert np.array_equal(k, want, equal_nan=True) and np.array_equal(v, want, equal_nan=True)
+    other = gen.standard_normal((9, 1, 64)).astype(np.float32)
+    for k, v in ((x, x), (x, other), (other, x)):
+        c = Cache(gen, 64, 1, 1, 1)
+        c.append(aa.F32, _dev(k), _dev(v), [0, 9], [9])
+        got = c.read(aa.F32, [0, 9], [9])
+        for g, want in zip(got, plain.pair_stands_for(k, v)):
+            assert np.isnan(want[3:7]).all() and np.isfinite(want[:3]).all() and np.isfinite(want[7:]).all()
+            assert np.array_equal(g, want.astype(np.float32).astype(np.float64), equal_nan=True)
 
 
 def test_append_leaves_the_rest_alone():
@@ -424,6 +427,10 @@ def test_attention_strides_types_of_rows_and_untouched_memory(rows, lens):
         _check(c, ty, q, st, lens, heads, 0.2, 0, out, lse)
         for mr in (1, 17, 1000):
             o2, l2 = _attend(c, ty, q, st, lens, heads, 0.2, max_rows=mr, out_stride=wide)
+            for b, r in enumerate(rows):  # rows past max_rows: NaN
+                over = slice(int(st[b]) + min(r, mr), int(st[b + 1]))
+                assert torch.isnan(o2[over, :heads * dim]).all() and torch.isnan(l2[over]).all()
+                o2[over], l2[over] = out[over], lse[over]
             _check(c, ty, q, st, lens, heads, 0.2, 0, o2, l2)
         o3, l3 = _attend(c, ty, q, st, lens, heads, 0.2, out_stride=wide, want_lse=False)
         assert (o3 == out).all() and (l3 == 7).all()
@@ -498,7 +505,7 @@ def test_attention_bad_row_starts_are_bounded():
     gen = np.random.default_rng(6)
     c = _filled(gen, 64, 1, [50, 50, 50])
     q = _dev(gen.standard_normal((4, 128)).astype(np.float32))
-    out, lse = _attend(c, aa.F32, q, [-3, 2, 1, 900], [50, 50, 50], 2, 0.1, max_rows=2)
+    out, lse = _attend(c, aa.F32, q, [-3, 2, 1, 900], [50, 50, 50], 2, 0.1, max_rows=4)
     # Row 1 is also sequence 2's (it starts there); row 0 is sequence 0's alone, one before its last.
     ok, ol = out.clone(), lse.clone()
     k, v = c.all([50, 50, 50])[0]
@@ -561,7 +568,7 @@ def test_slot_weights(case, ty):
         m = min(n, stride)
         k, v = c.all(lens)[b]
         w = plain.weights(hq[r1 - r:r1], k, hl[r1 - r:r1], scale, window)[:, :m] if r else np.zeros((kv, m))
-        size = np.abs(hq[r1 - r:r1]).max(initial=0) * np.abs(k).max(initial=0) * dim * scale  # at least sum |q k|
+        size = np.abs(hq[r1 - r:r1]).max(initial=0) * plain.parts(k).max(initial=0) * dim * scale if n else 0.0  # at least sum |q| parts
         for got, base in zip(results, (first[b], first[b], np.zeros_like(first[b]))):
             want = base[:, :m] + w
             bound = w * (2.0 ** -19 * size + 2.0 ** -20 + (heads // kv * max(r, 1) + 8) * U) + U * np.abs(want) + 1e-30
