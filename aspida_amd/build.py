@@ -35,7 +35,8 @@ CFLAGS = [
 # kv4_attn.hip: without it the decode attention's sums sit in AGPRs beside its
 # 192 VGPRs (228 in all, now 196).
 EXTRA_FLAGS = {"kq_mv_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
-               "kv4_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+               "kv4_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+               "kv4_weigh.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _compile(src):
