@@ -331,8 +331,9 @@ int aspida_kv4_attn_dev(const aspida_kv4 *cache, int type, const void *q, long l
  * lse: acc_out[b][g][j] = acc_in[b][g][j] + the sum over b's rows that see j
  * and the query heads of kv head g of exp(scale * q . k_j - lse), nothing for
  * slots from kv_len[b] on; both [n_seq][n_kv][acc_stride], slots past
- * acc_stride being left out.  acc_in may be acc_out, or NULL for zeros.  The
- * same bits every time (no atomics). */
+ * acc_stride being left out.  acc_in may be acc_out, or NULL for zeros.
+ * max_rows: at least the rows of the longest sequence (one with more gives
+ * NaN to the slots it sees).  The same bits every time (no atomics). */
 int aspida_kv4_weigh_dev(const aspida_kv4 *cache, int type, const void *q, long long q_stride, int n_heads, int n_rows,
                          int n_seq, const int *row_start, int max_rows, const int *kv_len, float scale, int window,
                          const float *lse, const float *acc_in, float *acc_out, long long acc_stride, void *stream);

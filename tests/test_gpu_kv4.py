@@ -577,6 +577,25 @@ def test_slot_weights(case, ty):
             assert np.array_equal(got[b][:, m:], base[:, m:])  # slots behind the length
 
 
+def test_slot_weights_with_too_small_max_rows():
+    """A sequence with more rows than max_rows gives NaN, the others are right."""
+    torch = torch_cuda()
+    gen = np.random.default_rng(3)
+    c = _filled(gen, 128, 1, [100, 80])
+    q = _dev(gen.standard_normal((6, 2 * 128)).astype(np.float32))
+    for rows, mr in (([5, 1], 1), ([1, 5], 4)):
+        st = _starts(rows)
+        _, lse = _attend(c, aa.F32, q, st, [100, 80], 2, 0.1)
+        out = torch.zeros(2, 1, 128, device="cuda")
+        s, l = _i32(st), _i32([100, 80])
+        c.dev.kv4_weigh(c.c, aa.F32, q.data_ptr(), 256, 2, 6, 2, s.data_ptr(), mr, l.data_ptr(), 0.1, lse.data_ptr(), 0,
+                        out.data_ptr(), 128, stream())
+        sync()
+        bad = 0 if rows[0] == 5 else 1
+        o = _host(out)[:, 0]
+        assert np.isnan(o[bad, :[96, 76][bad]]).all() and np.abs(o[1 - bad].sum() - 2) < 1e-4
+
+
 EVICTS = [
     # dim, kv, lens, keep, first, recent
     (128, 2, [200, 64, 10, 0], 64, 4, 16),
