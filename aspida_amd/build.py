@@ -36,7 +36,8 @@ CFLAGS = [
 # 192 VGPRs (228 in all, now 196).
 EXTRA_FLAGS = {"kq_mv_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
                "kv4_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
-               "kv4_weigh.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+               "kv4_weigh.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+               "kv4_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _compile(src):

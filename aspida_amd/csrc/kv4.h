@@ -74,6 +74,11 @@ size_t kv4_attn_work_bytes(int head_dim, int n_kv, int n_heads, int n_rows, int 
 hipError_t launch_kv4_attn(int head_dim, const Kv4View& c, int type, const Kv4Rows& rows, const Kv4Attn& a,
                            hipStream_t s);
 
+// Attention of many rows (kv4_prefill.hip), without a workspace.
+bool kv4_prefill_takes(const Kv4View& c, const Kv4Rows& rows, const Kv4Attn& a);
+hipError_t launch_kv4_prefill(int head_dim, const Kv4View& c, int type, const Kv4Rows& rows, const Kv4Attn& a,
+                              hipStream_t s);
+
 struct Kv4Weigh {
   const void* q;
   long long q_stride;

@@ -358,6 +358,7 @@ static void attn_typed(int head_dim, const SplitArgs& s, hipStream_t st) {
 
 hipError_t launch_kv4_attn(int head_dim, const Kv4View& c, int type, const Kv4Rows& rows, const Kv4Attn& a,
                            hipStream_t st) {
+  if (kv4_prefill_takes(c, rows, a)) return launch_kv4_prefill(head_dim, c, type, rows, a, st);
   SplitArgs s{c, rows, a, a.n_heads / c.n_kv, attn_tiles(a.n_heads / c.n_kv, a.max_rows)};
   if (type == ACT_F32) attn_typed<float>(head_dim, s, st);
   else if (type == ACT_F16) attn_typed<_Float16>(head_dim, s, st);

@@ -1,0 +1,401 @@
+// kv4_prefill.hip -- attention of many rows over the 4-bit cache.
+//
+// A workgroup takes 32 columns (rows times query heads of one kv head) per
+// wave and walks the pages that they see.  The waves turn a page's codes into
+// f16 operands in LDS once (exact, kv4_mma.h), in the order the 32x32x16
+// instructions read them, while the page before is multiplied; per 32 tokens
+//   S[token][col] = K Q^T      D / 16 steps, and one for the minima
+//   P = exp2(S - ref)          ref moves when a score passes it by 2^15
+//   O[dim][col] += V^T P       P in S's own registers: the steps' token order
+//                              is the one in which S's lanes hold them
+//   M[g][col] += m^T P         the minima, with a row of ones that sums P
+// f32 activations: two f16 planes of Q and of P, each in turn.
+// Bound by the matrix cores and exp2: a 32 x 32 tile of S is 19 steps of 32
+// cycles (D = 128, one plane) against about 400 cycles of vector work.
+#include <algorithm>
+
+#include "kv4_mma.h"
+
+namespace kq {
+
+__device__ __forceinline__ kvf16 kv_mfma32(kvh8 a, kvh8 b, kvf16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// LDS of one page: operands of 1 KB (a lane's eight halves at 16 lane).
+template <int D> struct PageLds {
+  static constexpr int NG = D / 32;
+  static constexpr int K = 0;                    // [32 tokens][D / 16 steps]
+  static constexpr int V = K + 128 * D;          // [32 tokens][D / 32 dim tiles][2 steps]
+  static constexpr int KM = V + 128 * D;         // minima of keys: [64 tokens][8]
+  static constexpr int VM = KM + 1024;           // of values: [32 tokens][2 steps][2 lane halves][16 rows]
+  static constexpr int BYTES = VM + 2048;
+};
+
+// What a thread loads of a page and later writes to LDS.
+template <int D, int THREADS> struct PageLoad {
+  static constexpr int NG = D / 32, QG = Kv4L<D>::QG;
+  static constexpr int KTASKS = 4 * 64 * (NG / QG), VTASKS = 2 * 64 * (D / 64);
+  static constexpr int KN = (KTASKS + THREADS - 1) / THREADS, VN = (VTASKS + THREADS - 1) / THREADS;
+  uint32_t kw[KN][QG], ks[KN][QG / 2];
+  kvu4 vw[VN], vd[VN][2];
+  kvu4 m;
+  bool there;
+
+  __device__ __forceinline__ void load(const Kv4View& c, int b, int p, int hk) {
+    using L = Kv4L<D>;
+    const uint8_t* blk = kv4_block(c, b, p, hk, L::BYTES);
+    there = blk != nullptr;
+    if (!blk) blk = c.pages;  // any page: its steps and minima become 0 below
+#pragma unroll
+    for (int i = 0; i < KN; ++i) {
+      const int t = threadIdx.x + i * THREADS;
+      if (KTASKS % THREADS && t >= KTASKS) continue;
+      const int lane = t & 63, quad = (t >> 6) % (NG / QG), tile = (t >> 6) / (NG / QG);
+      const uint8_t* w = blk + tile * L::KT + quad * (256 * QG) + lane * (4 * QG);
+      const uint8_t* s = blk + L::KS0 + (tile * 16 + (lane & 15)) * (4 * NG) + quad * (2 * QG);
+      __builtin_memcpy(kw[i], __builtin_assume_aligned(w, 4 * QG), 4 * QG);
+      __builtin_memcpy(ks[i], __builtin_assume_aligned(s, 2 * QG), 2 * QG);
+    }
+#pragma unroll
+    for (int i = 0; i < VN; ++i) {
+      const int t = threadIdx.x + i * THREADS;
+      if (VTASKS % THREADS && t >= VTASKS) continue;
+      const int lane = t & 63, ch = (t >> 6) % (D / 64), half = (t >> 6) / (D / 64);
+      vw[i] = *reinterpret_cast<const kvu4*>(blk + L::V0 + half * L::VB + ch * 1024 + lane * 16);
+      const uint8_t* s = blk + L::VS0 + half * L::VSB + (2 * ch) * 64 + (lane >> 4) * 16;
+      vd[i][0] = *reinterpret_cast<const kvu4*>(s);
+      vd[i][1] = *reinterpret_cast<const kvu4*>(s + 64);
+    }
+    // Minima: thread t < 64 of token t's key, then a piece of the values'.
+    const int t = threadIdx.x;
+    m = kvu4{0, 0, 0, 0};
+    if (t < 64) {
+      uint32_t r[4] = {0, 0, 0, 0};
+      __builtin_memcpy(r, __builtin_assume_aligned(blk + L::KS0 + t * (4 * NG) + 2 * NG, 4), 2 * NG);
+      m = kvu4{r[0], r[1], r[2], r[3]};
+    } else if (t < 64 + 8 * NG) {
+      const int u = t - 64, rg = u & 3, g = (u >> 2) % NG, half = (u >> 2) / NG;
+      m = *reinterpret_cast<const kvu4*>(blk + L::VS0 + half * L::VSB + 64 * NG + g * 64 + rg * 16);
+    }
+  }
+
+  // Steps and minima of value tokens outside [lo, hi) (of the page) become 0.
+  static __device__ __forceinline__ kvu4 keep(kvu4 d, int half, int rg, int lo, int hi) {
+    uint32_t r[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int t = 32 * half + 16 * (j >> 1) + 4 * rg + 2 * (j & 1);
+      r[j] = d[j] & ((t >= lo && t < hi ? 0x0000FFFFu : 0u) | (t + 1 >= lo && t + 1 < hi ? 0xFFFF0000u : 0u));
+    }
+    return kvu4{r[0], r[1], r[2], r[3]};
+  }
+
+  __device__ __forceinline__ void store(uint8_t* lds, int lo, int hi) {
+    using P = PageLds<D>;
+    if (!there) hi = 0;
+    const bool cut = lo > 0 || hi < KV4_PAGE;
+#pragma unroll
+    for (int i = 0; i < KN; ++i) {
+      const int t = threadIdx.x + i * THREADS;
+      if (KTASKS % THREADS && t >= KTASKS) continue;
+      const int lane = t & 63, quad = (t >> 6) % (NG / QG), tile = (t >> 6) / (NG / QG);
+      const int tok = tile * 16 + (lane & 15), kg = lane >> 4;
+      // Token tok % 32's dims 32 g + 8 kg ..: step 2 g + kg / 2, lane half kg % 2.
+      uint8_t* to = lds + P::K + (tok >> 5) * (64 * D) + ((kg & 1) * 32 + (tok & 31)) * 16;
+#pragma unroll
+      for (int g = 0; g < QG; ++g) {
+        const kvh2 pair = kv_h2(ks[i][g >> 1]);
+        const kvh2 d = (g & 1) ? __builtin_shufflevector(pair, pair, 1, 1) : __builtin_shufflevector(pair, pair, 0, 0);
+        *reinterpret_cast<kvh8*>(to + (2 * (quad * QG + g) + (kg >> 1)) * 1024) = kv4_unpack1(kw[i][g], d);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VN; ++i) {
+      const int t = threadIdx.x + i * THREADS;
+      if (VTASKS % THREADS && t >= VTASKS) continue;
+      const int lane = t & 63, ch = (t >> 6) % (D / 64), half = (t >> 6) / (D / 64), rg = lane >> 4;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const kvu4 dd = cut ? keep(vd[i][e], half, rg, lo, hi) : vd[i][e];
+        const kvh2 d0 = kv_h2(dd[0]), d1 = kv_h2(dd[1]), d2 = kv_h2(dd[2]), d3 = kv_h2(dd[3]);
+        const kvh2 n0 = kv_times(d0, -16.f), n1 = kv_times(d1, -256.f), n2 = kv_times(d2, -16.f), n3 = kv_times(d3, -256.f);
+        // Dims 64 ch + 32 e + 16 f + lane % 16 are dim tile 2 ch + e; tokens 4 rg .. of the first 16 are
+        // lane half rg % 2's, place rg / 2, of step 0, those of the other 16 of step 1.
+        uint8_t* to = lds + P::V + half * (64 * D) + (2 * ch + e) * 2048 + ((rg & 1) * 32 + (lane & 15)) * 16 + (rg >> 1) * 8;
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          const kvh8 v = kv4_unpack(vw[i][2 * e + f], d0, d1, d2, d3, n0, n1, n2, n3);
+          *reinterpret_cast<kvh4*>(to + f * 256) = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+          *reinterpret_cast<kvh4*>(to + f * 256 + 1024) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+        }
+      }
+    }
+    const int t = threadIdx.x;
+    if (t < 64) {
+      *reinterpret_cast<kvu4*>(lds + P::KM + t * 16) = m;
+    } else if (t < 64 + 8 * NG) {
+      const int u = t - 64, rg = u & 3, g = (u >> 2) % NG, half = (u >> 2) / NG;
+      const kvu4 mm = cut ? keep(m, half, rg, lo, hi) : m;
+      uint8_t* to = lds + P::VM + half * 1024 + ((rg & 1) * 16 + g) * 16 + (rg >> 1) * 8;
+      *reinterpret_cast<kvu2*>(to) = kvu2{mm[0], mm[1]};
+      *reinterpret_cast<kvu2*>(to + 512) = kvu2{mm[2], mm[3]};
+    }
+  }
+};
+
+struct PrefillArgs {
+  Kv4View c;
+  Kv4Rows rows;
+  Kv4Attn a;
+  int group;
+};
+
+constexpr float PF_LOG2E = 1.4426950408889634f, PF_LN2 = 0.6931471805599453f;
+
+template <int D, class T, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(PrefillArgs s) {
+  using P = PageLds<D>;
+  constexpr bool TWO = sizeof(T) == 4;
+  constexpr int NG = D / 32, NS = D / 16, THREADS = 64 * WAVES, COLS = 32 * WAVES;
+  extern __shared__ uint8_t lds[];  // two pages
+  const int lane = threadIdx.x & 63, col = lane & 31, hl = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hk = blockIdx.x, b = blockIdx.z;
+  const Kv4Span sp = kv4_span(s.rows, b);
+  const int n = sp.r1 - sp.r0, nr = min(n, s.a.max_rows);
+  // The last rows, which see most, come first.
+  const int tiles = (int)(((long long)nr * s.group + COLS - 1) / COLS), tile = tiles - 1 - (int)blockIdx.y;
+  if (tile < 0) return;
+  const int c0 = tile * COLS, c1 = min(c0 + COLS, nr * s.group);  // the workgroup's columns
+  const int first = sp.len - n;                                   // slot of row 0
+  const int max_slots = s.c.max_pages * KV4_PAGE;
+  const int any_hi = min(first + (c1 - 1) / s.group + 1, max_slots);
+  const int any_lo = s.a.window > 0 ? max(0, first + c0 / s.group - s.a.window + 1) : 0;
+
+  // This lane's column, and what the wave's columns all see and see at all.
+  const int w0 = c0 + 32 * wave, w1 = min(w0 + 32, c1) - 1;
+  const int ci = w0 + col, row = ci / s.group, head = hk * s.group + ci % s.group;
+  const bool valid = ci < c1;
+  const int pos = first + row;
+  const int chi = valid ? max(pos + 1, 0) : 0, clo = s.a.window > 0 ? max(0, pos - s.a.window + 1) : 0;
+  const int wave_hi = w0 <= w1 ? min(first + w1 / s.group + 1, max_slots) : 0;
+  const int wave_lo = s.a.window > 0 ? max(0, first + w0 / s.group - s.a.window + 1) : 0;
+  const int all_hi = first + w0 / s.group + 1;
+  const int all_lo = s.a.window > 0 ? max(0, first + max(w1, w0) / s.group - s.a.window + 1) : 0;
+
+  kvh8 qh[NS], ql[TWO ? NS : 1], qs;
+  float unit;
+  {
+    const T* q = (const T*)s.a.q + (size_t)(sp.r0 + (valid ? row : 0)) * s.a.q_stride + (size_t)head * D + 8 * hl;
+    float top = 0.f;
+    bool finite = true;
+    if (valid) {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        float x[8];
+        kv_load8(q + 16 * i, x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          top = fmaxf(top, fabsf(x[j]));
+          finite = finite && __builtin_isfinite(x[j]);
+        }
+      }
+    }
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    int e = 10;
+    if (top > 0.f && top <= 3.402823466e38f) e = __builtin_amdgcn_frexp_expf(top);
+    unit = finite ? ldexpf(1.f, e - 10) : __builtin_nanf("");
+    unit += 0.f * __shfl_xor(unit, 32, 64);
+    unit *= s.a.scale * PF_LOG2E;
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) qs[j] = (_Float16)0.f;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (valid) kv_load8(q + 16 * i, x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float c = ldexpf(finite ? x[j] : 0.f, 10 - e);
+        qh[i][j] = (_Float16)c;
+        if constexpr (TWO) ql[i][j] = (_Float16)(c - (float)qh[i][j]);
+        sum += c;
+      }
+      if (i & 1) {
+        sum += __shfl_xor(sum, 32, 64);
+        const _Float16 h = (_Float16)sum;
+        qs[i >> 1] = hl == 0 ? h : (_Float16)(sum - (float)h);
+        sum = 0.f;
+      }
+    }
+  }
+
+  kvf16 o[NG], om;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) om[i] = 0.f;
+#pragma unroll
+  for (int i = 0; i < NG; ++i) o[i] = om;
+  // A row past the table sees its own slot there: NaN.
+  float ref = -3.402823466e38f;
+  // The ones row sums P as the products see it, which is what o is divided by;
+  // with one plane those are rounded weights, and lse takes the unrounded sum.
+  float lsum = 0.f;
+  const bool past = chi > max_slots;
+
+  // Rows of the value minima that no group has: zeros, and ones in row 8.
+  for (int i = threadIdx.x; i < 2 * 2 * 64; i += THREADS) {
+    const int r = i & 15, u = (i >> 4) & 7, buf = i >> 7;
+    const uint32_t v = r == 8 ? 0x3C003C00u : 0u;
+    if (r >= NG) *reinterpret_cast<kvu4*>(lds + buf * P::BYTES + P::VM + (u * 16 + r) * 16) = kvu4{v, v, v, v};
+  }
+  const int p0 = any_lo / KV4_PAGE, p1 = any_hi > any_lo ? (any_hi - 1) / KV4_PAGE : p0 - 1;
+  PageLoad<D, THREADS> raw;
+  bool there = true, next_there = true;
+  auto store = [&](int p) {
+    raw.store(lds + (p & 1) * P::BYTES, any_lo - p * KV4_PAGE, any_hi - p * KV4_PAGE);
+    next_there = raw.there;
+  };
+  if (p0 <= p1) {
+    raw.load(s.c, b, p0, hk);
+    store(p0);
+    if (p0 < p1) raw.load(s.c, b, p0 + 1, hk);
+  }
+  for (int p = p0; p <= p1; ++p) {
+    there = next_there;
+    __syncthreads();
+    if (p < p1) {
+      store(p + 1);
+      if (p + 1 < p1) raw.load(s.c, b, p + 2, hk);
+    }
+    const uint8_t* pg = lds + (p & 1) * P::BYTES;
+    const int t0 = p * KV4_PAGE;
+    if (t0 >= wave_hi || t0 + KV4_PAGE <= wave_lo) continue;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = t0 + 32 * h;
+      if (at >= wave_hi || at + 32 <= wave_lo) continue;
+      kvf16 c;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) c[i] = 0.f;
+      c = kv_mfma32(*reinterpret_cast<const kvh8*>(pg + P::KM + (32 * h + col) * 16), qs, c);
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const kvh8 a = *reinterpret_cast<const kvh8*>(pg + P::K + h * (64 * D) + i * 1024 + lane * 16);
+        if constexpr (TWO) c = kv_mfma32(a, ql[i], c);
+        c = kv_mfma32(a, qh[i], c);
+      }
+      c *= unit;
+      if (!there || at + 32 > all_hi || at < all_lo) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int slot = at + 8 * (i >> 2) + 4 * hl + (i & 3);
+          c[i] = slot >= clo && slot < chi ? (there ? c[i] : __builtin_nanf("")) : -INFINITY;
+        }
+      }
+      float top = c[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, c[i]);
+      if (__ballot(top > ref + 15.f)) {
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float next = fmaxf(ref, top - 7.f), f = __builtin_amdgcn_exp2f(ref - next);
+        ref = next;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) o[i] *= f;
+        om *= f;
+        lsum *= f;
+      }
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        kvh8 ph, pl;
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[j] = __builtin_amdgcn_exp2f(c[8 * st + j] - ref);
+          ph[j] = (_Float16)x[j];
+          if constexpr (TWO) pl[j] = (_Float16)(x[j] - (float)ph[j]);
+        }
+        if constexpr (!TWO)
+          if (s.a.lse)
+            lsum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        const kvh8 m = *reinterpret_cast<const kvh8*>(pg + P::VM + h * 1024 + st * 512 + (hl * 16 + (col & 15)) * 16);
+        if constexpr (TWO) om = kv_mfma32(m, pl, om);
+        om = kv_mfma32(m, ph, om);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const kvh8 v = *reinterpret_cast<const kvh8*>(pg + P::V + h * (64 * D) + g * 2048 + st * 1024 + lane * 16);
+          if constexpr (TWO) o[g] = kv_mfma32(v, pl, o[g]);
+          o[g] = kv_mfma32(v, ph, o[g]);
+        }
+      }
+    }
+  }
+
+  // l is row 8 of om (lane half 0, register 4), group g's minima row g.
+  float l = __shfl(om[4], col, 64);
+  if (past) l = __builtin_nanf("");
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  T* out = (T*)s.a.out + (size_t)(sp.r0 + row) * s.a.out_stride + (size_t)head * D + 4 * hl;
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    const float m = __shfl(om[g & 3], ((g >> 2) & 1) * 32 + col, 64);
+    if (!valid) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      struct { T v[4]; } r;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r.v[j] = (T)((o[g][4 * i + j] + m) * inv);
+      __builtin_memcpy(out + 32 * g + 8 * i, &r, sizeof(r));
+    }
+  }
+  if (!TWO) l = lsum + __shfl_xor(lsum, 32, 64) + (past ? l : 0.f);
+  if (valid && s.a.lse && hl == 0)
+    s.a.lse[(size_t)(sp.r0 + row) * s.a.n_heads + head] = l != 0.f ? (ref + __builtin_amdgcn_logf(l)) * PF_LN2 : -INFINITY;
+  // Rows past max_rows have no workgroup: NaN, by the first tile's.
+  if (n > nr && tile == 0) {
+    const int w = s.group * D;
+    for (int r = sp.r0 + nr; r < sp.r1; ++r) {
+      for (int i = threadIdx.x; i < w; i += THREADS)
+        ((T*)s.a.out)[(size_t)r * s.a.out_stride + (size_t)hk * w + i] = (T)__builtin_nanf("");
+      if (s.a.lse && (int)threadIdx.x < s.group)
+        for (int i = threadIdx.x; i < s.group; i += THREADS)
+          s.a.lse[(size_t)r * s.a.n_heads + hk * s.group + i] = __builtin_nanf("");
+    }
+  }
+}
+
+template <int D, class T, int WAVES>
+static hipError_t prefill_go(const PrefillArgs& s, hipStream_t st) {
+  constexpr int lds = 2 * PageLds<D>::BYTES;
+  const hipError_t e = hipFuncSetAttribute((const void*)&kv4_prefill<D, T, WAVES>,
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (e != hipSuccess) return e;
+  const long long tiles = ((long long)std::min(s.a.max_rows, s.rows.n_rows) * s.group + 32 * WAVES - 1) / (32 * WAVES);
+  hipLaunchKernelGGL((kv4_prefill<D, T, WAVES>), dim3(s.c.n_kv, (unsigned)tiles, s.rows.n_seq), dim3(64 * WAVES), lds, st, s);
+  return hipGetLastError();
+}
+
+template <class T>
+static hipError_t prefill_typed(int head_dim, const PrefillArgs& s, hipStream_t st) {
+  if (head_dim == 64) return prefill_go<64, T, 8>(s, st);
+  if (head_dim == 128) return prefill_go<128, T, 8>(s, st);
+  return prefill_go<256, T, 4>(s, st);
+}
+
+// Many rows: enough columns to fill the 32 of a wave several times over, and
+// workgroups for most of the card (the split kernel cuts the slots instead).
+bool kv4_prefill_takes(const Kv4View& c, const Kv4Rows& rows, const Kv4Attn& a) {
+  const long long cols = (long long)std::min(a.max_rows, rows.n_rows) * (a.n_heads / c.n_kv);
+  const long long tiles = (cols + 255) / 256;
+  return cols >= 96 && tiles <= 65535 && tiles * c.n_kv * rows.n_seq >= 1;
+}
+
+hipError_t launch_kv4_prefill(int head_dim, const Kv4View& c, int type, const Kv4Rows& rows, const Kv4Attn& a,
+                              hipStream_t st) {
+  const PrefillArgs s{c, rows, a, a.n_heads / c.n_kv};
+  if (type == ACT_F32) return prefill_typed<float>(head_dim, s, st);
+  if (type == ACT_F16) return prefill_typed<_Float16>(head_dim, s, st);
+  return prefill_typed<bf16_t>(head_dim, s, st);
+}
+
+}  // namespace kq
