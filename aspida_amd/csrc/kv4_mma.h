@@ -28,6 +28,17 @@ __device__ __forceinline__ kvh8 kv4_unpack(uint32_t w, kvh2 d0, kvh2 d1, kvh2 d2
 }
 __device__ __forceinline__ kvh2 kv_times(kvh2 a, float s) { return a * kvh2{(_Float16)s, (_Float16)s}; }
 
+// The same less 8 steps, d (q - 8): -24 d takes the offset off, so every code
+// stands at the bits of 16 + q.
+__device__ __forceinline__ kvh8 kv4_unpack_centered(uint32_t w, kvh2 d0, kvh2 d1, kvh2 d2, kvh2 d3) {
+  const uint32_t r = __builtin_amdgcn_alignbit(w, w, 8);
+  const kvh2 a = kv_fma2(kv_h2((w & 0x03C003C0u) | 0x4C004C00u), d0, kv_times(d0, -24.f));
+  const kvh2 b = kv_fma2(kv_h2(((w << 4) & 0x03C003C0u) | 0x4C004C00u), d1, kv_times(d1, -24.f));
+  const kvh2 c = kv_fma2(kv_h2((r & 0x03C003C0u) | 0x4C004C00u), d2, kv_times(d2, -24.f));
+  const kvh2 e = kv_fma2(kv_h2(((r << 4) & 0x03C003C0u) | 0x4C004C00u), d3, kv_times(d3, -24.f));
+  return kvh8{a.x, a.y, b.x, b.y, c.x, c.y, e.x, e.y};
+}
+
 // Eight codes that share the step d2 = (d, d).
 __device__ __forceinline__ kvh8 kv4_unpack1(uint32_t w, kvh2 d2) {
   const kvh2 n16 = kv_times(d2, -16.f), n256 = kv_times(d2, -256.f);

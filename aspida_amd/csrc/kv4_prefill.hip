@@ -9,7 +9,10 @@
 //   O[dim][col] += V^T P       P in S's own registers: the steps' token order
 //                              is the one in which S's lanes hold them
 //   M[g][col] += m^T P         the minima, with a row of ones that sums P
-// f32 activations: two f16 planes of Q and of P, each in turn.
+// f32 activations: two f16 planes of Q and of P, each in turn, and value codes
+// less 8 (d (q - 8), with m + 8 d as two f16 in place of m): the sums over
+// thousands of slots then stay near the result instead of cancelling against
+// the minima (6000 slots: error 3.1e-6 before, of 1.5e-6 in plain f32).
 // Bound by the matrix cores and exp2: a 32 x 32 tile of S is 19 steps of 32
 // cycles (D = 128, one plane) against about 400 cycles of vector work.
 #include <algorithm>
@@ -23,23 +26,24 @@ __device__ __forceinline__ kvf16 kv_mfma32(kvh8 a, kvh8 b, kvf16 c) {
 }
 
 // LDS of one page: operands of 1 KB (a lane's eight halves at 16 lane).
-template <int D> struct PageLds {
+template <int D, bool TWO> struct PageLds {
   static constexpr int NG = D / 32;
   static constexpr int K = 0;                    // [32 tokens][D / 16 steps]
   static constexpr int V = K + 128 * D;          // [32 tokens][D / 32 dim tiles][2 steps]
   static constexpr int KM = V + 128 * D;         // minima of keys: [64 tokens][8]
   static constexpr int VM = KM + 1024;           // of values: [32 tokens][2 steps][2 lane halves][16 rows]
-  static constexpr int BYTES = VM + 2048;
+  static constexpr int VL = VM + 2048;           // what m + 8 d leaves after its f16 (f32 activations)
+  static constexpr int BYTES = VL + (TWO ? 2048 : 0);
 };
 
 // What a thread loads of a page and later writes to LDS.
-template <int D, int THREADS> struct PageLoad {
+template <int D, bool TWO, int THREADS> struct PageLoad {
   static constexpr int NG = D / 32, QG = Kv4L<D>::QG;
   static constexpr int KTASKS = 4 * 64 * (NG / QG), VTASKS = 2 * 64 * (D / 64);
   static constexpr int KN = (KTASKS + THREADS - 1) / THREADS, VN = (VTASKS + THREADS - 1) / THREADS;
   uint32_t kw[KN][QG], ks[KN][QG / 2];
   kvu4 vw[VN], vd[VN][2];
-  kvu4 m;
+  kvu4 m, md;
   bool there;
 
   __device__ __forceinline__ void load(const Kv4View& c, int b, int p, int hk) {
@@ -76,7 +80,9 @@ template <int D, int THREADS> struct PageLoad {
       m = kvu4{r[0], r[1], r[2], r[3]};
     } else if (t < 64 + 8 * NG) {
       const int u = t - 64, rg = u & 3, g = (u >> 2) % NG, half = (u >> 2) / NG;
-      m = *reinterpret_cast<const kvu4*>(blk + L::VS0 + half * L::VSB + 64 * NG + g * 64 + rg * 16);
+      const uint8_t* q = blk + L::VS0 + half * L::VSB + g * 64 + rg * 16;
+      m = *reinterpret_cast<const kvu4*>(q + 64 * NG);
+      if constexpr (TWO) md = *reinterpret_cast<const kvu4*>(q);
     }
   }
 
@@ -92,7 +98,7 @@ template <int D, int THREADS> struct PageLoad {
   }
 
   __device__ __forceinline__ void store(uint8_t* lds, int lo, int hi) {
-    using P = PageLds<D>;
+    using P = PageLds<D, TWO>;
     if (!there) hi = 0;
     const bool cut = lo > 0 || hi < KV4_PAGE;
 #pragma unroll
@@ -119,13 +125,14 @@ template <int D, int THREADS> struct PageLoad {
       for (int e = 0; e < 2; ++e) {
         const kvu4 dd = cut ? keep(vd[i][e], half, rg, lo, hi) : vd[i][e];
         const kvh2 d0 = kv_h2(dd[0]), d1 = kv_h2(dd[1]), d2 = kv_h2(dd[2]), d3 = kv_h2(dd[3]);
-        const kvh2 n0 = kv_times(d0, -16.f), n1 = kv_times(d1, -256.f), n2 = kv_times(d2, -16.f), n3 = kv_times(d3, -256.f);
         // Dims 64 ch + 32 e + 16 f + lane % 16 are dim tile 2 ch + e; tokens 4 rg .. of the first 16 are
         // lane half rg % 2's, place rg / 2, of step 0, those of the other 16 of step 1.
         uint8_t* to = lds + P::V + half * (64 * D) + (2 * ch + e) * 2048 + ((rg & 1) * 32 + (lane & 15)) * 16 + (rg >> 1) * 8;
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
-          const kvh8 v = kv4_unpack(vw[i][2 * e + f], d0, d1, d2, d3, n0, n1, n2, n3);
+          const kvh8 v = TWO ? kv4_unpack_centered(vw[i][2 * e + f], d0, d1, d2, d3)
+                             : kv4_unpack(vw[i][2 * e + f], d0, d1, d2, d3, kv_times(d0, -16.f), kv_times(d1, -256.f),
+                                          kv_times(d2, -16.f), kv_times(d3, -256.f));
           *reinterpret_cast<kvh4*>(to + f * 256) = __builtin_shufflevector(v, v, 0, 1, 2, 3);
           *reinterpret_cast<kvh4*>(to + f * 256 + 1024) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
         }
@@ -136,8 +143,22 @@ template <int D, int THREADS> struct PageLoad {
       *reinterpret_cast<kvu4*>(lds + P::KM + t * 16) = m;
     } else if (t < 64 + 8 * NG) {
       const int u = t - 64, rg = u & 3, g = (u >> 2) % NG, half = (u >> 2) / NG;
-      const kvu4 mm = cut ? keep(m, half, rg, lo, hi) : m;
+      kvu4 mm = cut ? keep(m, half, rg, lo, hi) : m;
       uint8_t* to = lds + P::VM + half * 1024 + ((rg & 1) * 16 + g) * 16 + (rg >> 1) * 8;
+      if constexpr (TWO) {
+        const kvu4 dd = cut ? keep(md, half, rg, lo, hi) : md;
+        uint32_t low[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const kvh2 mj = kv_h2(mm[j]), dj = kv_h2(dd[j]);
+          const float a = __builtin_fmaf(8.f, (float)dj.x, (float)mj.x), b = __builtin_fmaf(8.f, (float)dj.y, (float)mj.y);
+          const kvh2 hi2 = {(_Float16)a, (_Float16)b}, lo2 = {(_Float16)(a - (float)hi2.x), (_Float16)(b - (float)hi2.y)};
+          mm[j] = __builtin_bit_cast(uint32_t, hi2);
+          low[j] = __builtin_bit_cast(uint32_t, lo2);
+        }
+        *reinterpret_cast<kvu2*>(to + 2048) = kvu2{low[0], low[1]};
+        *reinterpret_cast<kvu2*>(to + 2048 + 512) = kvu2{low[2], low[3]};
+      }
       *reinterpret_cast<kvu2*>(to) = kvu2{mm[0], mm[1]};
       *reinterpret_cast<kvu2*>(to + 512) = kvu2{mm[2], mm[3]};
     }
@@ -155,8 +176,8 @@ constexpr float PF_LOG2E = 1.4426950408889634f, PF_LN2 = 0.6931471805599453f;
 
 template <int D, class T, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(PrefillArgs s) {
-  using P = PageLds<D>;
   constexpr bool TWO = sizeof(T) == 4;
+  using P = PageLds<D, TWO>;
   constexpr int NG = D / 32, NS = D / 16, THREADS = 64 * WAVES, COLS = 32 * WAVES;
   extern __shared__ uint8_t lds[];  // two pages
   const int lane = threadIdx.x & 63, col = lane & 31, hl = lane >> 5;
@@ -207,7 +228,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(Pr
     if (top > 0.f && top <= 3.402823466e38f) e = __builtin_amdgcn_frexp_expf(top);
     unit = finite ? ldexpf(1.f, e - 10) : __builtin_nanf("");
     unit += 0.f * __shfl_xor(unit, 32, 64);
-    unit *= s.a.scale * PF_LOG2E;
+    // unit stays positive (the largest score is the largest product): a
+    // negative scale turns the query round.
+    unit *= fabsf(s.a.scale) * PF_LOG2E;
+    const float turn = s.a.scale < 0.f ? -1.f : 1.f;
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) qs[j] = (_Float16)0.f;
@@ -217,7 +241,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(Pr
       if (valid) kv_load8(q + 16 * i, x);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float c = ldexpf(finite ? x[j] : 0.f, 10 - e);
+        const float c = ldexpf(finite ? x[j] : 0.f, 10 - e) * turn;
         qh[i][j] = (_Float16)c;
         if constexpr (TWO) ql[i][j] = (_Float16)(c - (float)qh[i][j]);
         sum += c;
@@ -247,10 +271,14 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(Pr
   for (int i = threadIdx.x; i < 2 * 2 * 64; i += THREADS) {
     const int r = i & 15, u = (i >> 4) & 7, buf = i >> 7;
     const uint32_t v = r == 8 ? 0x3C003C00u : 0u;
-    if (r >= NG) *reinterpret_cast<kvu4*>(lds + buf * P::BYTES + P::VM + (u * 16 + r) * 16) = kvu4{v, v, v, v};
+    if (r >= NG) {
+      uint8_t* to = lds + buf * P::BYTES + P::VM + (u * 16 + r) * 16;
+      *reinterpret_cast<kvu4*>(to) = kvu4{v, v, v, v};
+      if constexpr (TWO) *reinterpret_cast<kvu4*>(to + 2048) = kvu4{0, 0, 0, 0};
+    }
   }
   const int p0 = any_lo / KV4_PAGE, p1 = any_hi > any_lo ? (any_hi - 1) / KV4_PAGE : p0 - 1;
-  PageLoad<D, THREADS> raw;
+  PageLoad<D, TWO, THREADS> raw;
   bool there = true, next_there = true;
   auto store = [&](int p) {
     raw.store(lds + (p & 1) * P::BYTES, any_lo - p * KV4_PAGE, any_hi - p * KV4_PAGE);
@@ -285,17 +313,19 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(Pr
         if constexpr (TWO) c = kv_mfma32(a, ql[i], c);
         c = kv_mfma32(a, qh[i], c);
       }
-      c *= unit;
+      float u = unit;
       if (!there || at + 32 > all_hi || at < all_lo) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int slot = at + 8 * (i >> 2) + 4 * hl + (i & 3);
-          c[i] = slot >= clo && slot < chi ? (there ? c[i] : __builtin_nanf("")) : -INFINITY;
+          c[i] = slot >= clo && slot < chi ? (there ? c[i] * unit : __builtin_nanf("")) : -INFINITY;
         }
+        u = 1.f;
       }
       float top = c[0];
 #pragma unroll
       for (int i = 1; i < 16; ++i) top = fmaxf(top, c[i]);
+      top *= u;
       if (__ballot(top > ref + 15.f)) {
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         const float next = fmaxf(ref, top - 7.f), f = __builtin_amdgcn_exp2f(ref - next);
@@ -311,7 +341,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(Pr
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          x[j] = __builtin_amdgcn_exp2f(c[8 * st + j] - ref);
+          x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(c[8 * st + j], u, -ref));
           ph[j] = (_Float16)x[j];
           if constexpr (TWO) pl[j] = (_Float16)(x[j] - (float)ph[j]);
         }
@@ -319,7 +349,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(Pr
           if (s.a.lse)
             lsum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
         const kvh8 m = *reinterpret_cast<const kvh8*>(pg + P::VM + h * 1024 + st * 512 + (hl * 16 + (col & 15)) * 16);
-        if constexpr (TWO) om = kv_mfma32(m, pl, om);
+        if constexpr (TWO) {
+          const kvh8 m2 = *reinterpret_cast<const kvh8*>(pg + P::VL + h * 1024 + st * 512 + (hl * 16 + (col & 15)) * 16);
+          om = kv_mfma32(m2, ph, om);
+          om = kv_mfma32(m, pl, om);
+        }
         om = kv_mfma32(m, ph, om);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
@@ -366,7 +400,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(Pr
 
 template <int D, class T, int WAVES>
 static hipError_t prefill_go(const PrefillArgs& s, hipStream_t st) {
-  constexpr int lds = 2 * PageLds<D>::BYTES;
+  constexpr int lds = 2 * PageLds<D, sizeof(T) == 4>::BYTES;
   const hipError_t e = hipFuncSetAttribute((const void*)&kv4_prefill<D, T, WAVES>,
                                            hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) return e;
