@@ -45,6 +45,23 @@ __device__ __forceinline__ kvh8 kv4_unpack1(uint32_t w, kvh2 d2) {
   return kv4_unpack(w, d2, d2, d2, d2, n16, n256, n16, n256);
 }
 
+// The page ids of a sequence, 64 at a time in a wave's lanes: a lookup in a
+// loop is a lane read, where a scalar load would make every LDS wait of the
+// loop wait for it too.  Wave-uniform arguments.
+struct PageIds {
+  int ids, base;
+  __device__ __forceinline__ void fill(const Kv4View& c, int b, int p, int lane) {
+    base = p;
+    ids = p + lane < c.max_pages ? c.table[(size_t)b * c.max_pages + p + lane] : -1;
+  }
+  // kv4_block for p >= the base of the first fill, ascending.
+  __device__ __forceinline__ uint8_t* block(const Kv4View& c, int b, int p, int hk, int head_bytes, int lane) {
+    if (p - base >= 64) fill(c, b, p, lane);
+    const int id = __builtin_amdgcn_readlane(ids, p - base);
+    return (unsigned)id < (unsigned)c.n_pages ? c.pages + ((size_t)id * c.n_kv + hk) * head_bytes : nullptr;
+  }
+};
+
 // A lane's words of a 16-token key tile: token lane % 16, lane group kg =
 // lane / 16 of each group's dims; scales: all d of the token, then all m.
 template <int D> struct KeyTile {

@@ -25,139 +25,154 @@ __device__ __forceinline__ kvf16 kv_mfma32(kvh8 a, kvh8 b, kvf16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-// LDS of one page: operands of 1 KB (a lane's eight halves at 16 lane).
-template <int D, bool TWO> struct PageLds {
+// LDS of one stage, 32 tokens: operands of 1 KB (a lane's eight halves at 16 lane).
+template <int D, bool TWO> struct StageLds {
   static constexpr int NG = D / 32;
-  static constexpr int K = 0;                    // [32 tokens][D / 16 steps]
-  static constexpr int V = K + 128 * D;          // [32 tokens][D / 32 dim tiles][2 steps]
-  static constexpr int KM = V + 128 * D;         // minima of keys: [64 tokens][8]
-  static constexpr int VM = KM + 1024;           // of values: [32 tokens][2 steps][2 lane halves][16 rows]
-  static constexpr int VL = VM + 2048;           // what m + 8 d leaves after its f16 (f32 activations)
-  static constexpr int BYTES = VL + (TWO ? 2048 : 0);
+  static constexpr int K = 0;                    // [D / 16 steps]
+  static constexpr int V = K + 64 * D;           // [D / 32 dim tiles][2 steps]
+  static constexpr int KM = V + 64 * D;          // minima of keys: [32 tokens][8]
+  static constexpr int VM = KM + 512;            // of values: [2 steps][2 lane halves][16 rows][8]
+  static constexpr int VL = VM + 1024;           // what m + 8 d leaves after its f16 (f32 activations)
+  static constexpr int BYTES = VL + (TWO ? 1024 : 0);
 };
 
-// What a thread loads of a page and later writes to LDS.
-template <int D, bool TWO, int THREADS> struct PageLoad {
-  static constexpr int NG = D / 32, QG = Kv4L<D>::QG;
-  static constexpr int KTASKS = 4 * 64 * (NG / QG), VTASKS = 2 * 64 * (D / 64);
-  static constexpr int KN = (KTASKS + THREADS - 1) / THREADS, VN = (VTASKS + THREADS - 1) / THREADS;
-  uint32_t kw[KN][QG], ks[KN][QG / 2];
-  kvu4 vw[VN], vd[VN][2];
-  kvu4 m, md;
+// What a thread loads of a stage and later writes to LDS.  128 threads have
+// the keys, 128 the values; with eight waves, four take the even stages and
+// four the odd ones, so of the two waves of a SIMD one unpacks at a time.
+// Both halves load by the same instructions at offsets of their own: with a
+// branch the compiler joins the two halves' registers by moves, which wait
+// for the loads at once.
+template <int D, bool TWO> struct StageLoad {
+  static constexpr int NG = D / 32, QG = Kv4L<D>::QG, HALF = 128;
+  static constexpr int KTASKS = 2 * 64 * (NG / QG), VTASKS = D;
+  static constexpr int KN = KTASKS / HALF, VN = (VTASKS + HALF - 1) / HALF, N = KN > VN ? KN : VN;
+  // Keys: w the code words, d the steps of their token (from group 0).
+  // Values: w the code words of four 16-dim tiles, d and d2 the tokens' steps
+  // of their two groups.
+  kvu4 w[N], d[N], d2[N];
+  kvu4 m, md;  // a piece of the minima (and of the steps that go with it)
+  int ow[N], od[N], om;
   bool there;
 
-  __device__ __forceinline__ void load(const Kv4View& c, int b, int p, int hk) {
+  __device__ __forceinline__ void place(bool values, int tid) {
     using L = Kv4L<D>;
-    const uint8_t* blk = kv4_block(c, b, p, hk, L::BYTES);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int t = tid + i * HALF, lane = t & 63, quad = (t >> 6) % (NG / QG), tile = (t >> 6) / (NG / QG);
+      const int ch = (t >> 6) % (D / 64);
+      ow[i] = values ? L::V0 + ch * 1024 + lane * 16 : tile * L::KT + quad * (256 * QG) + lane * (4 * QG);
+      od[i] = values ? L::VS0 + 2 * ch * 64 + (lane >> 4) * 16 : L::KS0 + (tile * 16 + (lane & 15)) * (4 * NG);
+    }
+    om = values ? L::VS0 + ((tid >> 2) % NG) * 64 + (tid & 3) * 16 + 64 * NG : L::KS0 + (tid & 31) * (4 * NG) + 2 * NG;
+  }
+  // blk: the stage's page, null where there is none.  (The second half of a
+  // page lies 16 D bytes on in the codes, 4 D in the scales, and 16 bytes from
+  // any of these offsets are in the block.)
+  __device__ __forceinline__ void load(const uint8_t* blk, const uint8_t* any, int half) {
     there = blk != nullptr;
-    if (!blk) blk = c.pages;  // any page: its steps and minima become 0 below
+    if (!blk) blk = any;  // its steps and minima become 0 below
+    const uint8_t *pw = blk + half * (16 * D), *ps = blk + half * (4 * D);
+    auto at = [](const uint8_t* q) {
+      kvu4 v;
+      __builtin_memcpy(&v, __builtin_assume_aligned(q, 4), 16);
+      return v;
+    };
 #pragma unroll
-    for (int i = 0; i < KN; ++i) {
-      const int t = threadIdx.x + i * THREADS;
-      if (KTASKS % THREADS && t >= KTASKS) continue;
-      const int lane = t & 63, quad = (t >> 6) % (NG / QG), tile = (t >> 6) / (NG / QG);
-      const uint8_t* w = blk + tile * L::KT + quad * (256 * QG) + lane * (4 * QG);
-      const uint8_t* s = blk + L::KS0 + (tile * 16 + (lane & 15)) * (4 * NG) + quad * (2 * QG);
-      __builtin_memcpy(kw[i], __builtin_assume_aligned(w, 4 * QG), 4 * QG);
-      __builtin_memcpy(ks[i], __builtin_assume_aligned(s, 2 * QG), 2 * QG);
+    for (int i = 0; i < N; ++i) {
+      w[i] = at(pw + ow[i]);
+      d[i] = at(ps + od[i]);
+      d2[i] = at(ps + od[i] + 64);
     }
-#pragma unroll
-    for (int i = 0; i < VN; ++i) {
-      const int t = threadIdx.x + i * THREADS;
-      if (VTASKS % THREADS && t >= VTASKS) continue;
-      const int lane = t & 63, ch = (t >> 6) % (D / 64), half = (t >> 6) / (D / 64);
-      vw[i] = *reinterpret_cast<const kvu4*>(blk + L::V0 + half * L::VB + ch * 1024 + lane * 16);
-      const uint8_t* s = blk + L::VS0 + half * L::VSB + (2 * ch) * 64 + (lane >> 4) * 16;
-      vd[i][0] = *reinterpret_cast<const kvu4*>(s);
-      vd[i][1] = *reinterpret_cast<const kvu4*>(s + 64);
-    }
-    // Minima: thread t < 64 of token t's key, then a piece of the values'.
-    const int t = threadIdx.x;
-    m = kvu4{0, 0, 0, 0};
-    if (t < 64) {
-      uint32_t r[4] = {0, 0, 0, 0};
-      __builtin_memcpy(r, __builtin_assume_aligned(blk + L::KS0 + t * (4 * NG) + 2 * NG, 4), 2 * NG);
-      m = kvu4{r[0], r[1], r[2], r[3]};
-    } else if (t < 64 + 8 * NG) {
-      const int u = t - 64, rg = u & 3, g = (u >> 2) % NG, half = (u >> 2) / NG;
-      const uint8_t* q = blk + L::VS0 + half * L::VSB + g * 64 + rg * 16;
-      m = *reinterpret_cast<const kvu4*>(q + 64 * NG);
-      if constexpr (TWO) md = *reinterpret_cast<const kvu4*>(q);
-    }
+    m = at(ps + om);
+    if constexpr (TWO) md = at(ps + om - 64 * NG + (om < Kv4L<D>::VS0 ? 64 * NG : 0));
   }
 
-  // Steps and minima of value tokens outside [lo, hi) (of the page) become 0.
-  static __device__ __forceinline__ kvu4 keep(kvu4 d, int half, int rg, int lo, int hi) {
+  // Steps and minima of value tokens outside [lo, hi) (of the stage) become 0.
+  static __device__ __forceinline__ kvu4 keep(kvu4 x, int rg, int lo, int hi) {
     uint32_t r[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int t = 32 * half + 16 * (j >> 1) + 4 * rg + 2 * (j & 1);
-      r[j] = d[j] & ((t >= lo && t < hi ? 0x0000FFFFu : 0u) | (t + 1 >= lo && t + 1 < hi ? 0xFFFF0000u : 0u));
+      const int t = 16 * (j >> 1) + 4 * rg + 2 * (j & 1);
+      r[j] = x[j] & ((t >= lo && t < hi ? 0x0000FFFFu : 0u) | (t + 1 >= lo && t + 1 < hi ? 0xFFFF0000u : 0u));
     }
     return kvu4{r[0], r[1], r[2], r[3]};
   }
 
-  __device__ __forceinline__ void store(uint8_t* lds, int lo, int hi) {
-    using P = PageLds<D, TWO>;
-    if (!there) hi = 0;
-    const bool cut = lo > 0 || hi < KV4_PAGE;
+  __device__ __forceinline__ void store(uint8_t* lds, int lo, int hi, bool values, int tid) {
+    using P = StageLds<D, TWO>;
+    if (!values) {
 #pragma unroll
-    for (int i = 0; i < KN; ++i) {
-      const int t = threadIdx.x + i * THREADS;
-      if (KTASKS % THREADS && t >= KTASKS) continue;
-      const int lane = t & 63, quad = (t >> 6) % (NG / QG), tile = (t >> 6) / (NG / QG);
-      const int tok = tile * 16 + (lane & 15), kg = lane >> 4;
-      // Token tok % 32's dims 32 g + 8 kg ..: step 2 g + kg / 2, lane half kg % 2.
-      uint8_t* to = lds + P::K + (tok >> 5) * (64 * D) + ((kg & 1) * 32 + (tok & 31)) * 16;
+      for (int i = 0; i < KN; ++i) {
+        const int t = tid + i * HALF, lane = t & 63, quad = (t >> 6) % (NG / QG), tile = (t >> 6) / (NG / QG);
+        const int tok = tile * 16 + (lane & 15), kg = lane >> 4;
+        // Token tok's dims 32 g + 8 kg ..: step 2 g + kg / 2, lane half kg % 2.
+        uint8_t* to = lds + P::K + ((kg & 1) * 32 + tok) * 16 + (kg >> 1) * 1024;
 #pragma unroll
-      for (int g = 0; g < QG; ++g) {
-        const kvh2 pair = kv_h2(ks[i][g >> 1]);
-        const kvh2 d = (g & 1) ? __builtin_shufflevector(pair, pair, 1, 1) : __builtin_shufflevector(pair, pair, 0, 0);
-        *reinterpret_cast<kvh8*>(to + (2 * (quad * QG + g) + (kg >> 1)) * 1024) = kv4_unpack1(kw[i][g], d);
+        for (int g = 0; g < QG; ++g) {
+          const uint32_t two = NG == 8 && quad ? d[i][2 + (g >> 1)] : d[i][g >> 1];
+          const kvh2 pair = kv_h2(two);
+          const kvh2 dd = (g & 1) ? __builtin_shufflevector(pair, pair, 1, 1) : __builtin_shufflevector(pair, pair, 0, 0);
+          *reinterpret_cast<kvh8*>(to + 2 * (quad * QG + g) * 1024) = kv4_unpack1(w[i][g], dd);
+        }
       }
+      // (What follows a token's minima is not its own.)  The scores of a page
+      // that is not there are NaN.
+      if constexpr (NG == 4) m = kvu4{m.x, m.y, 0, 0};
+      if constexpr (NG == 2) m = kvu4{m.x, 0, 0, 0};
+      if (!there) m = kvu4{0x7E007E00u, 0x7E007E00u, 0x7E007E00u, 0x7E007E00u};
+      if (tid < 32) *reinterpret_cast<kvu4*>(lds + P::KM + tid * 16) = m;
+      return;
+    }
+    if (!there) hi = 0;
+    const bool cut = lo > 0 || hi < 32;
+    if (cut) {
+#pragma unroll
+      for (int i = 0; i < VN; ++i) {
+        const int rg = (tid & 63) >> 4;
+        d[i] = keep(d[i], rg, lo, hi);
+        d2[i] = keep(d2[i], rg, lo, hi);
+      }
+      m = keep(m, tid & 3, lo, hi);
+      if constexpr (TWO) md = keep(md, tid & 3, lo, hi);
     }
 #pragma unroll
     for (int i = 0; i < VN; ++i) {
-      const int t = threadIdx.x + i * THREADS;
-      if (VTASKS % THREADS && t >= VTASKS) continue;
-      const int lane = t & 63, ch = (t >> 6) % (D / 64), half = (t >> 6) / (D / 64), rg = lane >> 4;
+      const int t = tid + i * HALF;
+      if (VTASKS % HALF && t >= VTASKS) continue;
+      const int lane = t & 63, ch = t >> 6, rg = lane >> 4;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const kvu4 dd = cut ? keep(vd[i][e], half, rg, lo, hi) : vd[i][e];
-        const kvh2 d0 = kv_h2(dd[0]), d1 = kv_h2(dd[1]), d2 = kv_h2(dd[2]), d3 = kv_h2(dd[3]);
+        const kvu4 dd = e ? d2[i] : d[i];
+        const kvh2 d0 = kv_h2(dd[0]), d1 = kv_h2(dd[1]), dd2 = kv_h2(dd[2]), d3 = kv_h2(dd[3]);
         // Dims 64 ch + 32 e + 16 f + lane % 16 are dim tile 2 ch + e; tokens 4 rg .. of the first 16 are
         // lane half rg % 2's, place rg / 2, of step 0, those of the other 16 of step 1.
-        uint8_t* to = lds + P::V + half * (64 * D) + (2 * ch + e) * 2048 + ((rg & 1) * 32 + (lane & 15)) * 16 + (rg >> 1) * 8;
+        uint8_t* to = lds + P::V + (2 * ch + e) * 2048 + ((rg & 1) * 32 + (lane & 15)) * 16 + (rg >> 1) * 8;
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
-          const kvh8 v = TWO ? kv4_unpack_centered(vw[i][2 * e + f], d0, d1, d2, d3)
-                             : kv4_unpack(vw[i][2 * e + f], d0, d1, d2, d3, kv_times(d0, -16.f), kv_times(d1, -256.f),
-                                          kv_times(d2, -16.f), kv_times(d3, -256.f));
+          const kvh8 v = TWO ? kv4_unpack_centered(w[i][2 * e + f], d0, d1, dd2, d3)
+                             : kv4_unpack(w[i][2 * e + f], d0, d1, dd2, d3, kv_times(d0, -16.f), kv_times(d1, -256.f),
+                                          kv_times(dd2, -16.f), kv_times(d3, -256.f));
           *reinterpret_cast<kvh4*>(to + f * 256) = __builtin_shufflevector(v, v, 0, 1, 2, 3);
           *reinterpret_cast<kvh4*>(to + f * 256 + 1024) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
         }
       }
     }
-    const int t = threadIdx.x;
-    if (t < 64) {
-      *reinterpret_cast<kvu4*>(lds + P::KM + t * 16) = m;
-    } else if (t < 64 + 8 * NG) {
-      const int u = t - 64, rg = u & 3, g = (u >> 2) % NG, half = (u >> 2) / NG;
-      kvu4 mm = cut ? keep(m, half, rg, lo, hi) : m;
-      uint8_t* to = lds + P::VM + half * 1024 + ((rg & 1) * 16 + g) * 16 + (rg >> 1) * 8;
+    if (tid < 4 * NG) {
+      const int rg = tid & 3, g = tid >> 2;
+      kvu4 mm = m;
+      uint8_t* to = lds + P::VM + ((rg & 1) * 16 + g) * 16 + (rg >> 1) * 8;
       if constexpr (TWO) {
-        const kvu4 dd = cut ? keep(md, half, rg, lo, hi) : md;
         uint32_t low[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const kvh2 mj = kv_h2(mm[j]), dj = kv_h2(dd[j]);
+          const kvh2 mj = kv_h2(mm[j]), dj = kv_h2(md[j]);
           const float a = __builtin_fmaf(8.f, (float)dj.x, (float)mj.x), b = __builtin_fmaf(8.f, (float)dj.y, (float)mj.y);
           const kvh2 hi2 = {(_Float16)a, (_Float16)b}, lo2 = {(_Float16)(a - (float)hi2.x), (_Float16)(b - (float)hi2.y)};
           mm[j] = __builtin_bit_cast(uint32_t, hi2);
           low[j] = __builtin_bit_cast(uint32_t, lo2);
         }
-        *reinterpret_cast<kvu2*>(to + 2048) = kvu2{low[0], low[1]};
-        *reinterpret_cast<kvu2*>(to + 2048 + 512) = kvu2{low[2], low[3]};
+        *reinterpret_cast<kvu2*>(to + 1024) = kvu2{low[0], low[1]};
+        *reinterpret_cast<kvu2*>(to + 1024 + 512) = kvu2{low[2], low[3]};
       }
       *reinterpret_cast<kvu2*>(to) = kvu2{mm[0], mm[1]};
       *reinterpret_cast<kvu2*>(to + 512) = kvu2{mm[2], mm[3]};
@@ -177,9 +192,9 @@ constexpr float PF_LOG2E = 1.4426950408889634f, PF_LN2 = 0.6931471805599453f;
 template <int D, class T, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(PrefillArgs s) {
   constexpr bool TWO = sizeof(T) == 4;
-  using P = PageLds<D, TWO>;
+  using P = StageLds<D, TWO>;
   constexpr int NG = D / 32, NS = D / 16, THREADS = 64 * WAVES, COLS = 32 * WAVES;
-  extern __shared__ uint8_t lds[];  // two pages
+  extern __shared__ uint8_t lds[];  // three stages, and the low plane of Q
   const int lane = threadIdx.x & 63, col = lane & 31, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hk = blockIdx.x, b = blockIdx.z;
@@ -200,12 +215,14 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(Pr
   const bool valid = ci < c1;
   const int pos = first + row;
   const int chi = valid ? max(pos + 1, 0) : 0, clo = s.a.window > 0 ? max(0, pos - s.a.window + 1) : 0;
-  const int wave_hi = w0 <= w1 ? min(first + w1 / s.group + 1, max_slots) : 0;
-  const int wave_lo = s.a.window > 0 ? max(0, first + w0 / s.group - s.a.window + 1) : 0;
   const int all_hi = first + w0 / s.group + 1;
   const int all_lo = s.a.window > 0 ? max(0, first + max(w1, w0) / s.group - s.a.window + 1) : 0;
 
-  kvh8 qh[NS], ql[TWO ? NS : 1], qs;
+  // f32 activations with a head of 128: the low plane of Q would not fit in
+  // the registers of two waves per SIMD and is read from LDS.
+  constexpr bool QL_LDS = TWO && WAVES == 8;
+  uint8_t* const qlds = lds + 3 * P::BYTES + wave * (NS * 1024) + lane * 16;
+  kvh8 qh[NS], ql[TWO && !QL_LDS ? NS : 1], qs;
   float unit;
   {
     const T* q = (const T*)s.a.q + (size_t)(sp.r0 + (valid ? row : 0)) * s.a.q_stride + (size_t)head * D + 8 * hl;
@@ -238,14 +255,17 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(Pr
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      kvh8 low;
       if (valid) kv_load8(q + 16 * i, x);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float c = ldexpf(finite ? x[j] : 0.f, 10 - e) * turn;
         qh[i][j] = (_Float16)c;
-        if constexpr (TWO) ql[i][j] = (_Float16)(c - (float)qh[i][j]);
+        if constexpr (TWO) low[j] = (_Float16)(c - (float)qh[i][j]);
         sum += c;
       }
+      if constexpr (QL_LDS) *reinterpret_cast<kvh8*>(qlds + i * 1024) = low;
+      else if constexpr (TWO) ql[i] = low;
       if (i & 1) {
         sum += __shfl_xor(sum, 32, 64);
         const _Float16 h = (_Float16)sum;
@@ -268,101 +288,138 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(Pr
   const bool past = chi > max_slots;
 
   // Rows of the value minima that no group has: zeros, and ones in row 8.
-  for (int i = threadIdx.x; i < 2 * 2 * 64; i += THREADS) {
-    const int r = i & 15, u = (i >> 4) & 7, buf = i >> 7;
+  for (int i = threadIdx.x; i < 3 * 64; i += THREADS) {
+    const int r = i & 15, u = (i >> 4) & 3, buf = i >> 6;
     const uint32_t v = r == 8 ? 0x3C003C00u : 0u;
     if (r >= NG) {
       uint8_t* to = lds + buf * P::BYTES + P::VM + (u * 16 + r) * 16;
       *reinterpret_cast<kvu4*>(to) = kvu4{v, v, v, v};
-      if constexpr (TWO) *reinterpret_cast<kvu4*>(to + 2048) = kvu4{0, 0, 0, 0};
+      if constexpr (TWO) *reinterpret_cast<kvu4*>(to + 1024) = kvu4{0, 0, 0, 0};
     }
   }
-  const int p0 = any_lo / KV4_PAGE, p1 = any_hi > any_lo ? (any_hi - 1) / KV4_PAGE : p0 - 1;
-  PageLoad<D, TWO, THREADS> raw;
-  bool there = true, next_there = true;
-  auto store = [&](int p) {
-    raw.store(lds + (p & 1) * P::BYTES, any_lo - p * KV4_PAGE, any_hi - p * KV4_PAGE);
-    next_there = raw.there;
+  // Stages [s0, s1), an even number (one past the end is all masked).  While
+  // stage s is multiplied by its weights, the scores of s + 1 are formed and
+  // stage s + 2 is unpacked into the buffer of s - 1.
+  const int s0 = any_lo / 32, s1 = any_hi > any_lo ? s0 + (((any_hi - 1) / 32 + 2 - s0) & ~1) : s0;
+  constexpr int TURNS = WAVES / 4;  // groups of four waves that take turns
+  StageLoad<D, TWO> raw;
+  const int turn = wave >> 2, tid = threadIdx.x & 127;
+  const bool values = wave & 2;
+  raw.place(values, tid);
+  auto store = [&](int st) {
+    raw.store(lds + (st % 3) * P::BYTES, any_lo - 32 * st, any_hi - 32 * st, values, tid);
   };
-  if (p0 <= p1) {
-    raw.load(s.c, b, p0, hk);
-    store(p0);
-    if (p0 < p1) raw.load(s.c, b, p0 + 1, hk);
-  }
-  for (int p = p0; p <= p1; ++p) {
-    there = next_there;
+  PageIds ids;
+  ids.fill(s.c, b, s0 >> 1, lane);
+  auto fetch = [&](int st) {
+    raw.load(st < s1 ? ids.block(s.c, b, st >> 1, hk, Kv4L<D>::BYTES, lane) : nullptr, s.c.pages, st & 1);
+  };
+  auto scores = [&](int st) {
+    const uint8_t* pg = lds + (st % 3) * P::BYTES;
+    kvf16 c;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) c[i] = 0.f;
+    c = kv_mfma32(*reinterpret_cast<const kvh8*>(pg + P::KM + col * 16), qs, c);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const kvh8 k = *reinterpret_cast<const kvh8*>(pg + P::K + i * 1024 + lane * 16);
+      if constexpr (QL_LDS) c = kv_mfma32(k, *reinterpret_cast<const kvh8*>(qlds + i * 1024), c);
+      else if constexpr (TWO) c = kv_mfma32(k, ql[i], c);
+      c = kv_mfma32(k, qh[i], c);
+    }
+    return c;
+  };
+  float u = unit;  // what c is to be multiplied by
+  // Masks the scores of a stage that not every column sees whole, and moves
+  // ref where a score passes it.
+  auto settle = [&](kvf16& c, int st) {
+    const int at = 32 * st;
+    u = unit;
+    if (at + 32 > all_hi || at < all_lo) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int slot = at + 8 * (i >> 2) + 4 * hl + (i & 3);
+        c[i] = slot >= clo && slot < chi ? c[i] * unit : -INFINITY;
+      }
+      u = 1.f;
+    }
+    float top = c[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, c[i]);
+    top *= u;
+    if (__ballot(top > ref + 15.f)) {
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float next = fmaxf(ref, top - 7.f), f = __builtin_amdgcn_exp2f(ref - next);
+      ref = next;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) o[i] *= f;
+      om *= f;
+      lsum *= f;
+    }
+  };
+  // One stage: its weights from the scores c, the next one's scores into c2.
+  auto step = [&](int st, const kvf16& c, kvf16& c2) {
+    const uint8_t* pg = lds + (st % 3) * P::BYTES;
+    c2 = scores(min(st + 1, s1 - 1));
+    kvh8 ph[2], pl[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(c[8 * e + j], u, -ref));
+        ph[e][j] = (_Float16)x[j];
+        if constexpr (TWO) pl[e][j] = (_Float16)(x[j] - (float)ph[e][j]);
+      }
+      if constexpr (!TWO) lsum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const kvh8 vm = *reinterpret_cast<const kvh8*>(pg + P::VM + e * 512 + (hl * 16 + (col & 15)) * 16);
+      if constexpr (TWO) {
+        const kvh8 vl = *reinterpret_cast<const kvh8*>(pg + P::VL + e * 512 + (hl * 16 + (col & 15)) * 16);
+        om = kv_mfma32(vl, ph[e], om);
+        om = kv_mfma32(vm, pl[e], om);
+      }
+      om = kv_mfma32(vm, ph[e], om);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const kvh8 v = *reinterpret_cast<const kvh8*>(pg + P::V + g * 2048 + e * 1024 + lane * 16);
+        if constexpr (TWO) o[g] = kv_mfma32(v, pl[e], o[g]);
+        o[g] = kv_mfma32(v, ph[e], o[g]);
+      }
+    }
     __syncthreads();
-    if (p < p1) {
-      store(p + 1);
-      if (p + 1 < p1) raw.load(s.c, b, p + 2, hk);
+    settle(c2, min(st + 1, s1 - 1));
+  };
+  kvf16 ca, cb;
+  if (s0 < s1) {
+    if constexpr (TURNS == 1) {
+      fetch(s0);
+      store(s0);
+      fetch(s0 + 1);
+      store(s0 + 1);
+      fetch(s0 + 2);
+    } else {
+      fetch(s0 + turn);
+      store(s0 + turn);
+      fetch(s0 + 2 + turn);
     }
-    const uint8_t* pg = lds + (p & 1) * P::BYTES;
-    const int t0 = p * KV4_PAGE;
-    if (t0 >= wave_hi || t0 + KV4_PAGE <= wave_lo) continue;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int at = t0 + 32 * h;
-      if (at >= wave_hi || at + 32 <= wave_lo) continue;
-      kvf16 c;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) c[i] = 0.f;
-      c = kv_mfma32(*reinterpret_cast<const kvh8*>(pg + P::KM + (32 * h + col) * 16), qs, c);
-#pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        const kvh8 a = *reinterpret_cast<const kvh8*>(pg + P::K + h * (64 * D) + i * 1024 + lane * 16);
-        if constexpr (TWO) c = kv_mfma32(a, ql[i], c);
-        c = kv_mfma32(a, qh[i], c);
-      }
-      float u = unit;
-      if (!there || at + 32 > all_hi || at < all_lo) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int slot = at + 8 * (i >> 2) + 4 * hl + (i & 3);
-          c[i] = slot >= clo && slot < chi ? (there ? c[i] * unit : __builtin_nanf("")) : -INFINITY;
-        }
-        u = 1.f;
-      }
-      float top = c[0];
-#pragma unroll
-      for (int i = 1; i < 16; ++i) top = fmaxf(top, c[i]);
-      top *= u;
-      if (__ballot(top > ref + 15.f)) {
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float next = fmaxf(ref, top - 7.f), f = __builtin_amdgcn_exp2f(ref - next);
-        ref = next;
-#pragma unroll
-        for (int i = 0; i < NG; ++i) o[i] *= f;
-        om *= f;
-        lsum *= f;
-      }
-#pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        kvh8 ph, pl;
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(c[8 * st + j], u, -ref));
-          ph[j] = (_Float16)x[j];
-          if constexpr (TWO) pl[j] = (_Float16)(x[j] - (float)ph[j]);
-        }
-        if constexpr (!TWO)
-          if (s.a.lse)
-            lsum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-        const kvh8 m = *reinterpret_cast<const kvh8*>(pg + P::VM + h * 1024 + st * 512 + (hl * 16 + (col & 15)) * 16);
-        if constexpr (TWO) {
-          const kvh8 m2 = *reinterpret_cast<const kvh8*>(pg + P::VL + h * 1024 + st * 512 + (hl * 16 + (col & 15)) * 16);
-          om = kv_mfma32(m2, ph, om);
-          om = kv_mfma32(m, pl, om);
-        }
-        om = kv_mfma32(m, ph, om);
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          const kvh8 v = *reinterpret_cast<const kvh8*>(pg + P::V + h * (64 * D) + g * 2048 + st * 1024 + lane * 16);
-          if constexpr (TWO) o[g] = kv_mfma32(v, pl, o[g]);
-          o[g] = kv_mfma32(v, ph, o[g]);
-        }
-      }
-    }
+  }
+  __syncthreads();
+  if (s0 < s1) {
+    ca = scores(s0);
+    settle(ca, s0);
+  }
+  for (int st = s0; st < s1; st += 2) {
+    // The loads of both groups stand where each finds its registers free: the
+    // first group's have this stage to arrive, the second's two.
+    if (TURNS == 1 || turn == 0) store(st + 2);
+    if constexpr (TURNS == 1) fetch(st + 3);
+    step(st, ca, cb);
+    if (TURNS == 1 || turn == 1) store(st + 3);
+    fetch(TURNS == 1 ? st + 4 : st + 4 + turn);
+    step(st + 1, cb, ca);
   }
 
   // l is row 8 of om (lane half 0, register 4), group g's minima row g.
@@ -400,7 +457,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(Pr
 
 template <int D, class T, int WAVES>
 static hipError_t prefill_go(const PrefillArgs& s, hipStream_t st) {
-  constexpr int lds = 2 * PageLds<D, sizeof(T) == 4>::BYTES;
+  constexpr int lds = 3 * StageLds<D, sizeof(T) == 4>::BYTES + (sizeof(T) == 4 && WAVES == 8 ? WAVES * D * 64 : 0);
   const hipError_t e = hipFuncSetAttribute((const void*)&kv4_prefill<D, T, WAVES>,
                                            hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) return e;
