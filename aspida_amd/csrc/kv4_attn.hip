@@ -166,30 +166,32 @@ __global__ __launch_bounds__(64 * ATTN_WAVES) void kv4_attn_split(SplitArgs s) {
   // A row past the table sees its own slot there: NaN.
   float ref = REF0, l = chi > s.c.max_pages * KV4_PAGE && cut.index == 0 && wave == 0 ? __builtin_nanf("") : 0.f;
 
+  // Two sets of registers: one is multiplied while the other arrives.  The
+  // loads are the same every time (past the end they read any page again), so
+  // nothing makes the compiler move, and wait for, what is on its way.
+  struct Set {
+    KeyTile<D> k[2];
+    ValueBlock<D> v;
+    bool there;
+  };
   int t = t0 + 32 * wave;
-  KeyTile<D> k[2];
-  ValueBlock<D> v;
-  bool there = false;
-  auto load = [&](int at) {
-    const uint8_t* blk = kv4_block(s.c, b, at >> 6, hk, L::BYTES);
-    there = blk != nullptr;
+  PageIds ids;
+  ids.fill(s.c, b, t0 >> 6, lane);
+  auto load = [&](Set& x, int at) {
+    const uint8_t* blk = at < any_hi ? ids.block(s.c, b, at >> 6, hk, L::BYTES, lane) : nullptr;
+    x.there = blk != nullptr;
     if (!blk) blk = s.c.pages;  // any page: what is read there is not used
     const int half = (at >> 5) & 1;
-    k[0].load(blk, 2 * half, lane);
-    k[1].load(blk, 2 * half + 1, lane);
-    v.load(blk, half, lane);
+    x.k[0].load(blk, 2 * half, lane);
+    x.k[1].load(blk, 2 * half + 1, lane);
+    x.v.load(blk, half, lane);
   };
-  if (t < any_hi) load(t);
-  for (; t < any_hi; t += ATTN_STEP) {
-    kvf4 c[2] = {q.scores(k[0]), q.scores(k[1])};
+  auto step = [&](Set& y, int at) {
+    kvf4 c[2] = {q.scores(y.k[0]), q.scores(y.k[1])};
     float x[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = c[j >> 2][j & 3] * unit;
-    ValueBlock<D> vv = v;
-    const bool ok = there;
-    const int at = t;
-    if (t + ATTN_STEP < any_hi) load(t + ATTN_STEP);
-    if (!ok || at + 32 > all_hi || at < all_lo) {
+    if (!y.there || at + 32 > all_hi || at < all_lo) {
       // Slots that this column does not see get no weight; the steps and
       // minima of slots that no column sees may be anything and become 0.
       uint32_t keep = 0;
@@ -197,10 +199,10 @@ __global__ __launch_bounds__(64 * ATTN_WAVES) void kv4_attn_split(SplitArgs s) {
       for (int j = 0; j < 8; ++j) {
         const int slot = at + 16 * (j >> 2) + 4 * rg + (j & 3);
         const bool see = slot >= clo && slot < chi;
-        x[j] = see ? (ok ? x[j] : __builtin_nanf("")) : -INFINITY;
-        if (ok && slot < any_hi && slot >= any_lo) keep |= 1u << j;
+        x[j] = see ? (y.there ? x[j] : __builtin_nanf("")) : -INFINITY;
+        if (y.there && slot < any_hi && slot >= any_lo) keep |= 1u << j;
       }
-      vv.drop(keep);
+      y.v.drop(keep);
     }
     float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
     if (__ballot(top > ref + 15.f)) {
@@ -224,21 +226,30 @@ __global__ __launch_bounds__(64 * ATTN_WAVES) void kv4_attn_split(SplitArgs s) {
       ph[j] = (_Float16)p;
       if constexpr (TWO) pl[j] = (_Float16)(p - (float)ph[j]);
     }
-    const kvh8 vm = __builtin_bit_cast(kvh8, vv.m);
+    const kvh8 vm = __builtin_bit_cast(kvh8, y.v.m);
     if constexpr (TWO) om = kv_mfma(vm, pl, om);
     om = kv_mfma(vm, ph, om);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      const kvh2 d0 = kv_h2(vv.d[g][0]), d1 = kv_h2(vv.d[g][1]), d2 = kv_h2(vv.d[g][2]), d3 = kv_h2(vv.d[g][3]);
+      const kvh2 d0 = kv_h2(y.v.d[g][0]), d1 = kv_h2(y.v.d[g][1]), d2 = kv_h2(y.v.d[g][2]), d3 = kv_h2(y.v.d[g][3]);
       const kvh2 n0 = kv_times(d0, -16.f), n1 = kv_times(d1, -256.f), n2 = kv_times(d2, -16.f), n3 = kv_times(d3, -256.f);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int i = 2 * g + e;
-        const kvh8 a = kv4_unpack(vv.w[i >> 2][i & 3], d0, d1, d2, d3, n0, n1, n2, n3);
+        const kvh8 a = kv4_unpack(y.v.w[i >> 2][i & 3], d0, d1, d2, d3, n0, n1, n2, n3);
         if constexpr (TWO) o[i] = kv_mfma(a, pl, o[i]);
         o[i] = kv_mfma(a, ph, o[i]);
       }
     }
+  };
+  Set xa, xb;
+  if (t < any_hi) load(xa, t);
+  for (; t < any_hi; t += 2 * ATTN_STEP) {
+    load(xb, t + ATTN_STEP);
+    step(xa, t);
+    if (t + ATTN_STEP >= any_hi) break;
+    load(xa, t + 2 * ATTN_STEP);
+    step(xb, t + ATTN_STEP);
   }
 
   // The wave's column sums: l over the lane groups, and the minima's part of
@@ -274,7 +285,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES) void kv4_attn_split(SplitArgs s) {
   }
   if (wave != 0 || !valid) return;
   if (cut.count == 1) {
-    const float inv = l != 0.f ? 1.f / l : 0.f;
+    const float inv = l != 0.f ? 1.f / l : 0.f;  // NaN stays
     T* out = (T*)s.a.out + (size_t)(sp.r0 + row) * s.a.out_stride + (size_t)head * D;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -291,15 +302,18 @@ __global__ __launch_bounds__(64 * ATTN_WAVES) void kv4_attn_split(SplitArgs s) {
   if (rg == 0) { part->ref[col] = ref; part->l[col] = l; }
 }
 
-// Joins the chunks of a sequence: a workgroup per (kv head and column tile,
-// sequence), a wave per column in turn.
+// Joins the chunks of a sequence: a workgroup per (column of a kv head's
+// tile, sequence).  Each of its waves takes every fourth chunk, 64 lanes over
+// the dims; LDS adds the four up.
 template <int D, class T>
 __global__ __launch_bounds__(256) void kv4_attn_join(SplitArgs s) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int b = blockIdx.y, hk = blockIdx.x / s.tiles, tile = blockIdx.x % s.tiles;
+  constexpr int E = D / 64;
+  __shared__ float so[4][D], sl[4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = blockIdx.z, hk = blockIdx.y / s.tiles, tile = blockIdx.y % s.tiles, col = blockIdx.x;
   const Kv4Span sp = kv4_span(s.rows, b);
   const int ncol = min(16, min(sp.r1 - sp.r0, s.a.max_rows) * s.group - tile * 16);
-  if (ncol <= 0) return;
+  if (col >= ncol) return;
   const int slots = s.c.max_pages * KV4_PAGE;
   const int chunk = chunk_tokens(s.rows, s.a.window, slots, s.c.n_kv * s.tiles);
   const int count = chunks_of(s.rows, b, s.a.window, slots, chunk);
@@ -307,28 +321,32 @@ __global__ __launch_bounds__(256) void kv4_attn_join(SplitArgs s) {
   int first = 0;
   for (int i = lane; i < b; i += 64) first += chunks_of(s.rows, i, s.a.window, slots, chunk);
   for (int o = 32; o; o >>= 1) first += __shfl_xor(first, o, 64);
-  const AttnPart<D>* part = (const AttnPart<D>*)s.a.work + (size_t)first * gridDim.x + blockIdx.x;
-  const size_t step = gridDim.x;
-  for (int col = wave; col < ncol; col += 4) {
-    float ref = REF0;
-    for (int i = lane; i < count; i += 64) ref = fmaxf(ref, part[i * step].ref[col]);
-    for (int o = 32; o; o >>= 1) ref = fmaxf(ref, __shfl_xor(ref, o, 64));
-    float l = 0.f, y[D / 64] = {};
-    for (int i = 0; i < count; ++i) {
-      const AttnPart<D>& p = part[i * step];
-      const float f = __builtin_amdgcn_exp2f(p.ref[col] - ref);
-      l += p.l[col] * f;
+  const AttnPart<D>* part = (const AttnPart<D>*)s.a.work + (size_t)first * gridDim.y + blockIdx.y;
+  const size_t step = gridDim.y;
+  float ref = REF0;
+  for (int i = lane; i < count; i += 64) ref = fmaxf(ref, part[i * step].ref[col]);
+  for (int o = 32; o; o >>= 1) ref = fmaxf(ref, __shfl_xor(ref, o, 64));
+  float l = 0.f, y[E] = {};
+#pragma unroll 8
+  for (int i = wave; i < count; i += 4) {
+    const AttnPart<D>& p = part[i * step];
+    const float f = __builtin_amdgcn_exp2f(p.ref[col] - ref);
+    l += p.l[col] * f;
 #pragma unroll
-      for (int e = 0; e < D / 64; ++e) y[e] += p.o[col][lane + 64 * e] * f;
-    }
-    const int ci = tile * 16 + col, row = sp.r0 + ci / s.group, head = hk * s.group + ci % s.group;
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-#pragma unroll
-    for (int e = 0; e < D / 64; ++e)
-      ((T*)s.a.out)[(size_t)row * s.a.out_stride + (size_t)head * D + lane + 64 * e] = (T)(y[e] * inv);
-    if (s.a.lse && lane == 0)
-      s.a.lse[(size_t)row * s.a.n_heads + head] = l != 0.f ? (ref + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+    for (int e = 0; e < E; ++e) y[e] += p.o[col][lane * E + e] * f;
   }
+#pragma unroll
+  for (int e = 0; e < E; ++e) so[wave][lane * E + e] = y[e];
+  if (lane == 0) sl[wave] = l;
+  __syncthreads();
+  const int i = threadIdx.x;
+  if (i >= D) return;
+  l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+  const float v = (so[0][i] + so[1][i]) + (so[2][i] + so[3][i]);
+  const int ci = tile * 16 + col, row = sp.r0 + ci / s.group, head = hk * s.group + ci % s.group;
+  ((T*)s.a.out)[(size_t)row * s.a.out_stride + (size_t)head * D + i] = (T)(l != 0.f ? v / l : 0.f);
+  if (s.a.lse && i == 0)
+    s.a.lse[(size_t)row * s.a.n_heads + head] = l != 0.f ? (ref + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
 }
 
 static int attn_tiles(int group, int max_rows) { return (int)std::min<long long>(65535, ((long long)max_rows * group + 15) / 16); }
@@ -346,7 +364,8 @@ template <int D, class T>
 static void attn_go(const SplitArgs& s, hipStream_t st) {
   const int per_seq = s.c.n_kv * s.tiles;
   hipLaunchKernelGGL((kv4_attn_split<D, T>), dim3(attn_chunks(per_seq, s.rows.n_seq), per_seq), dim3(64 * ATTN_WAVES), 0, st, s);
-  hipLaunchKernelGGL((kv4_attn_join<D, T>), dim3(per_seq, s.rows.n_seq), dim3(256), 0, st, s);
+  const int cols = (int)std::min<long long>(16, (long long)s.a.max_rows * s.group);
+  hipLaunchKernelGGL((kv4_attn_join<D, T>), dim3(cols, per_seq, s.rows.n_seq), dim3(256), 0, st, s);
 }
 
 template <class T>
