@@ -16,9 +16,11 @@
 //                           the value dwords are ordered; one more step for
 //                           the minima
 // so nothing passes through LDS until the waves of a workgroup are joined.
-// A sequence's slots are cut into chunks of a length that all workgroups
-// derive from the lengths on the device (the host does not know them), so
-// that all chunks together fill the card; a second launch joins them.
+// The sequences' slots stand one after the other on one axis, which is cut
+// into equal shares, one for each workgroup that fits on the card at once: a
+// workgroup takes what of one sequence or of several lies in its share, and a
+// second launch joins the parts of a sequence.  All of it follows from the
+// lengths on the device, which the host does not know.
 #include <algorithm>
 
 #include "kv4_mma.h"
@@ -27,8 +29,15 @@ namespace kq {
 
 constexpr int ATTN_WAVES = 4;
 constexpr int ATTN_STEP = 32 * ATTN_WAVES;  // tokens of a workgroup's round
+// Tokens whose page ids a wave holds at once: whole rounds, within 64 pages
+// wherever in a page they start.
+constexpr int ATTN_SEGMENT = (4096 - 32) / ATTN_STEP * ATTN_STEP;
 // Workgroups that the chunks are cut for: three for each of 256 CUs.
-constexpr int ATTN_GROUPS = 768;
+// Workgroups that fit at once: 256 CUs times what their registers allow (134,
+// 198 and over 256 for heads of 64, 128 and 256).  One round of equal shares
+// measured against 1.5 and 2 rounds (32/8 heads, f32): 130001 slots 47, 59
+// and 57 us; 16 lanes of 8000 45, 56 and 54 us.
+template <int D> constexpr int ATTN_GROUPS = D == 64 ? 768 : D == 128 ? 512 : 256;
 constexpr float REF0 = -3.402823466e38f;  // below every score
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
@@ -43,55 +52,81 @@ __device__ __forceinline__ SeenRange seen_range(const Kv4Span& s, int window, in
   return r;
 }
 
-// How the sequences' slots are cut.  Every wave derives the same: chunk, the
-// tokens of a chunk, and for a workgroup number x its sequence and chunk
-// (seq < 0: none), with the sequence's chunks and the number of its first.
-struct Cut { int seq, index, count, first, chunk; };
+// A sequence's rounds (one at least: one whose rows see nothing has outputs
+// too), and its length on the axis, which counts what a workgroup spends on a
+// sequence besides: its rows, page ids and sums, about 8000 cycles where a
+// round takes 1800.
+constexpr int AXIS_EXTRA = 4;
+__device__ __forceinline__ int rounds_of(const Kv4Span& s, int window, int max_slots) {
+  const SeenRange r = seen_range(s, window, max_slots);
+  return max(1, (r.hi - r.lo + ATTN_STEP - 1) / ATTN_STEP);
+}
 
-__device__ __forceinline__ int chunk_tokens(const Kv4Rows& rows, int window, int max_slots, int per_seq) {
+// Where workgroup x's share starts: [x0, x0 + share) of the axis, sequence seq
+// (n_seq: none) from `start` of it on.
+struct AxisPlace { long long x0, share, start; int seq; };
+
+// Inclusive sum over the lanes.
+__device__ __forceinline__ long long wave_scan64(long long v) {
   const int lane = threadIdx.x & 63;
-  float total = 0.f;
-  for (int b = lane; b < rows.n_seq; b += 64) {
-    const SeenRange r = seen_range(kv4_span(rows, b), window, max_slots);
-    total += (float)max(r.hi - r.lo, 0);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const long long u = __shfl_up(v, o, 64);
+    if (lane >= o) v += u;
   }
-  total = wave_total(total) * (float)per_seq;
-  const float want = total / (float)ATTN_GROUPS;
-  const int steps = (int)fminf(ceilf(want / (float)ATTN_STEP), 8388608.f);
-  return max(1, steps) * ATTN_STEP;
+  return v;
 }
 
-__device__ __forceinline__ int chunks_of(const Kv4Rows& rows, int b, int window, int max_slots, int chunk) {
-  const SeenRange r = seen_range(kv4_span(rows, b), window, max_slots);
-  return max(1, (r.hi - r.lo + chunk - 1) / chunk);
-}
-
-__device__ __forceinline__ Cut cut_of(const Kv4Rows& rows, int window, int max_slots, int per_seq, int x) {
+// own: the span of sequence `lane`, which the first 64 sequences' lengths come
+// from.
+__device__ __forceinline__ long long axis_total(const Kv4Rows& rows, const Kv4Span& own, int window, int max_slots) {
   const int lane = threadIdx.x & 63;
-  Cut c;
-  c.chunk = chunk_tokens(rows, window, max_slots, per_seq);
-  int before = 0;
+  long long total = lane < rows.n_seq ? rounds_of(own, window, max_slots) + AXIS_EXTRA : 0;
+  for (int b = 64 + lane; b < rows.n_seq; b += 64) total += rounds_of(kv4_span(rows, b), window, max_slots) + AXIS_EXTRA;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o, 64);
+  return total;
+}
+
+__device__ __forceinline__ AxisPlace axis_place(const Kv4Rows& rows, const Kv4Span& own, int window, int max_slots,
+                                                int groups, int x) {
+  const int lane = threadIdx.x & 63;
+  AxisPlace p;
+  if (rows.n_seq <= 64) {  // one lane each, and sums below 2^30
+    const int n = lane < rows.n_seq ? rounds_of(own, window, max_slots) + AXIS_EXTRA : 0;
+    const int end = wave_scan_add(n);
+    p.share = (__builtin_amdgcn_readlane(end, 63) + groups - 1) / groups;
+    p.x0 = x * p.share;
+    const uint64_t over = __ballot(end > p.x0);
+    const int l = over ? __builtin_ctzll(over) : 63;
+    p.seq = over ? l : rows.n_seq;
+    p.start = __builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(n, l);
+    return p;
+  }
+  p.share = (axis_total(rows, own, window, max_slots) + groups - 1) / groups;
+  p.x0 = x * p.share;
+  long long before = 0;
   for (int b0 = 0; b0 < rows.n_seq; b0 += 64) {
-    const int n = b0 + lane < rows.n_seq ? chunks_of(rows, b0 + lane, window, max_slots, c.chunk) : 0;
-    const int end = before + wave_scan_add(n);
-    const uint64_t over = __ballot(end > x);
+    const int b = b0 + lane;
+    const int n = b < rows.n_seq ? rounds_of(b0 ? kv4_span(rows, b) : own, window, max_slots) + AXIS_EXTRA : 0;
+    const long long end = before + wave_scan64(n);
+    const uint64_t over = __ballot(end > p.x0);
     if (over) {
       const int l = __builtin_ctzll(over);
-      c.seq = b0 + l;
-      c.count = __builtin_amdgcn_readlane(n, l);
-      c.first = __builtin_amdgcn_readlane(end, l) - c.count;
-      c.index = x - c.first;
-      return c;
+      p.seq = b0 + l;
+      p.start = __shfl(end, l, 64) - __shfl(n, l, 64);
+      return p;
     }
-    before = __builtin_amdgcn_readlane(end, 63);
+    before = __shfl(end, 63, 64);
   }
-  c.seq = -1;
-  c.index = c.count = c.first = 0;
-  return c;
+  p.seq = rows.n_seq;
+  p.start = before;
+  return p;
 }
 
-// Workspace: per chunk, kv head and column tile the columns' sums [16][D] and
-// (ref, l) [16].
+// Workspace: per part, kv head and column tile the columns' sums [16][D] and
+// (ref, l) [16].  Workgroup x's part of sequence b is number x + b: along the
+// axis one or the other grows.
 template <int D> struct AttnPart {
   float o[16][D];
   float ref[16], l[16];
@@ -102,6 +137,7 @@ struct SplitArgs {
   Kv4Rows rows;
   Kv4Attn a;
   int group, tiles;  // query heads of a kv head, column tiles
+  int groups;        // workgroups that share the axis
 };
 
 template <class T>
@@ -126,184 +162,223 @@ __device__ void fill_excess(const SplitArgs& s, const Kv4Span& sp, int hk, int d
 }
 
 template <int D, class T>
-__global__ __launch_bounds__(64 * ATTN_WAVES) void kv4_attn_split(SplitArgs s) {
+__global__ __launch_bounds__(64 * ATTN_WAVES, D == 64 ? 3 : D == 128 ? 2 : 1) void kv4_attn_split(SplitArgs s) {
   using L = Kv4L<D>;
   constexpr bool TWO = sizeof(T) == 4;
   constexpr int NG = D / 32, NT = D / 16;
   __shared__ float so[2][16][D];
   __shared__ float sr[2][16], sl[2][16];
-  const int lane = threadIdx.x & 63, col = lane & 15, rg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Cut cut = cut_of(s.rows, s.a.window, s.c.max_pages * KV4_PAGE, s.c.n_kv * s.tiles, blockIdx.x);
-  if (cut.seq < 0) return;
-  const int b = cut.seq, hk = blockIdx.y / s.tiles, tile = blockIdx.y % s.tiles;
-  const Kv4Span sp = kv4_span(s.rows, b);
-  const int n = sp.r1 - sp.r0;
-  if (n > s.a.max_rows && cut.index == 0 && tile == 0) fill_excess<T>(s, sp, hk, D);
-  const int ncol = min(16, min(n, s.a.max_rows) * s.group - tile * 16);
-  if (ncol <= 0) return;
-  // This lane's column: its row, head, and the slots [clo, chi) it sees.
-  const int ci = tile * 16 + col, row = ci / s.group, head = hk * s.group + ci % s.group;
-  const bool valid = col < ncol;
-  const int pos = sp.len - n + row;
-  const int chi = valid ? max(pos + 1, 0) : 0, clo = s.a.window > 0 ? max(0, pos - s.a.window + 1) : 0;
-  Query<D, TWO> q;
-  q.load((const T*)s.a.q + (size_t)(sp.r0 + (valid ? row : 0)) * s.a.q_stride + (size_t)head * D, valid, lane);
-  const float unit = q.unit * (s.a.scale * LOG2E);
+  const int hk = blockIdx.y / s.tiles, tile = blockIdx.y % s.tiles;
+  const int max_slots = s.c.max_pages * KV4_PAGE;
+  // The first 64 sequences' spans, a lane each.
+  const int mine = threadIdx.x & 63;
+  Kv4Span own = {0, 0, 0};
+  if (mine < s.rows.n_seq) own = kv4_span(s.rows, mine);
+  AxisPlace place = axis_place(s.rows, own, s.a.window, max_slots, s.groups, blockIdx.x);
+  const long long x1 = place.x0 + place.share;
+  for (int b = place.seq; b < s.rows.n_seq && place.start < x1; ++b) {
+    // (Opaque, so that what follows from it is not kept in registers from one
+    // sequence to the next: 251 of them against 198.)
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    const int col = lane & 15, rg = lane >> 4;
+    Kv4Span sp;
+    if (b < 64) {
+      sp.r0 = __builtin_amdgcn_readlane(own.r0, b);
+      sp.r1 = __builtin_amdgcn_readlane(own.r1, b);
+      sp.len = __builtin_amdgcn_readlane(own.len, b);
+    } else {
+      sp = kv4_span(s.rows, b);
+    }
+    const SeenRange seen = seen_range(sp, s.a.window, max_slots);
+    const int length = rounds_of(sp, s.a.window, max_slots);
+    // Its rounds [u0, u1) are in this share.
+    const long long at = place.start + AXIS_EXTRA;
+    place.start = at + length;
+    const int u0 = (int)max(0ll, place.x0 - at), u1 = (int)min((long long)length, x1 - at);
+    const bool whole = u0 == 0 && u1 == length;
+    if (u0 >= u1) continue;
+    const int n = sp.r1 - sp.r0;
+    if (n > s.a.max_rows && u0 == 0 && tile == 0) fill_excess<T>(s, sp, hk, D);
+    const int ncol = min(16, min(n, s.a.max_rows) * s.group - tile * 16);
+    if (ncol <= 0) continue;
+    // This lane's column: its row, head, and the slots [clo, chi) it sees.
+    const int ci = tile * 16 + col, row = ci / s.group, head = hk * s.group + ci % s.group;
+    const bool valid = col < ncol;
+    const int pos = sp.len - n + row;
+    const int chi = valid ? max(pos + 1, 0) : 0, clo = s.a.window > 0 ? max(0, pos - s.a.window + 1) : 0;
+    // The share's slots, and those of them that every column sees.
+    const int t0 = seen.lo + u0 * ATTN_STEP, t1 = (int)min((long long)seen.hi, seen.lo + (long long)u1 * ATTN_STEP);
+    const int row_last = (tile * 16 + ncol - 1) / s.group, row_first = tile * 16 / s.group;
+    const int all_hi = sp.len - n + row_first + 1;                                       // below: seen by every column
+    const int all_lo = s.a.window > 0 ? max(0, sp.len - n + row_last - s.a.window + 1) : 0;
+    const int any_hi = min(t1, sp.len - n + row_last + 1);
+    const int any_lo = s.a.window > 0 ? max(0, sp.len - n + row_first - s.a.window + 1) : 0;
 
-  // The chunk's slots, and those of them that every column sees.
-  const SeenRange seen = seen_range(sp, s.a.window, s.c.max_pages * KV4_PAGE);
-  const int t0 = seen.lo + cut.index * cut.chunk, t1 = min(seen.hi, t0 + cut.chunk);
-  const int row_last = (tile * 16 + ncol - 1) / s.group, row_first = tile * 16 / s.group;
-  const int all_hi = sp.len - n + row_first + 1;                                       // below: seen by every column
-  const int all_lo = s.a.window > 0 ? max(0, sp.len - n + row_last - s.a.window + 1) : 0;
-  const int any_hi = min(t1, sp.len - n + row_last + 1);
-  const int any_lo = s.a.window > 0 ? max(0, sp.len - n + row_first - s.a.window + 1) : 0;
-
-  kvf4 o[NT], om = {0.f, 0.f, 0.f, 0.f};
+    kvf4 o[NT], om = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < NT; ++i) o[i] = om;
-  // A row past the table sees its own slot there: NaN.
-  float ref = REF0, l = chi > s.c.max_pages * KV4_PAGE && cut.index == 0 && wave == 0 ? __builtin_nanf("") : 0.f;
+    for (int i = 0; i < NT; ++i) o[i] = om;
+    // A row past the table sees its own slot there: NaN.
+    float ref = REF0, l = chi > max_slots && u0 == 0 && wave == 0 ? __builtin_nanf("") : 0.f;
 
-  // Two sets of registers: one is multiplied while the other arrives.  The
-  // loads are the same every time (past the end they read any page again), so
-  // nothing makes the compiler move, and wait for, what is on its way.
-  struct Set {
-    KeyTile<D> k[2];
-    ValueBlock<D> v;
-    bool there;
-  };
-  int t = t0 + 32 * wave;
-  PageIds ids;
-  ids.fill(s.c, b, t0 >> 6, lane);
-  auto load = [&](Set& x, int at) {
-    const uint8_t* blk = at < any_hi ? ids.block(s.c, b, at >> 6, hk, L::BYTES, lane) : nullptr;
-    x.there = blk != nullptr;
-    if (!blk) blk = s.c.pages;  // any page: what is read there is not used
-    const int half = (at >> 5) & 1;
-    x.k[0].load(blk, 2 * half, lane);
-    x.k[1].load(blk, 2 * half + 1, lane);
-    x.v.load(blk, half, lane);
-  };
-  auto step = [&](Set& y, int at) {
-    kvf4 c[2] = {q.scores(y.k[0]), q.scores(y.k[1])};
-    float x[8];
+    // Two sets of registers: one is multiplied while the other arrives.  The
+    // loads are the same every time (past the end they read any page again), so
+    // nothing makes the compiler move, and wait for, what is on its way.
+    struct Set {
+      KeyTile<D> k[2];
+      ValueBlock<D> v;
+      bool there;
+    };
+    PageIds ids;
+    int end = 0;
+    auto load = [&](Set& x, int at) {
+      const uint8_t* blk = at < end ? ids.at(s.c, at >> 6, hk, L::BYTES) : nullptr;
+      x.there = blk != nullptr;
+      if (!blk) blk = s.c.pages;  // any page: what is read there is not used
+      const int half = (at >> 5) & 1;
+      x.k[0].load(blk, 2 * half, lane);
+      x.k[1].load(blk, 2 * half + 1, lane);
+      x.v.load(blk, half, lane);
+    };
+    Query<D, TWO> q;
+    float unit;
+    auto step = [&](Set& y, int at) {
+      kvf4 c[2] = {q.scores(y.k[0]), q.scores(y.k[1])};
+      float x[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = c[j >> 2][j & 3] * unit;
-    if (!y.there || at + 32 > all_hi || at < all_lo) {
-      // Slots that this column does not see get no weight; the steps and
-      // minima of slots that no column sees may be anything and become 0.
-      uint32_t keep = 0;
+      for (int j = 0; j < 8; ++j) x[j] = c[j >> 2][j & 3];
+      float u = unit;
+      if (!y.there || at + 32 > all_hi || at < all_lo) {
+        // Slots that this column does not see get no weight; the steps and
+        // minima of slots that no column sees may be anything and become 0.
+        uint32_t keep = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int slot = at + 16 * (j >> 2) + 4 * rg + (j & 3);
+          const bool see = slot >= clo && slot < chi;
+          x[j] = see ? (y.there ? x[j] * unit : __builtin_nanf("")) : -INFINITY;
+          if (y.there && slot < any_hi && slot >= any_lo) keep |= 1u << j;
+        }
+        y.v.drop(keep);
+        u = 1.f;
+      }
+      float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * u;
+      if (__ballot(top > ref + 15.f)) {
+        // P' = exp2(x - ref) is kept below 2^15; after a move the maximum of the
+        // column is at 2^7.
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float next = fmaxf(ref, top - 7.f);
+        const float f = __builtin_amdgcn_exp2f(ref - next);
+        ref = next;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) o[i] *= f;
+        om *= f;
+      }
+      kvh8 ph, pl;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int slot = at + 16 * (j >> 2) + 4 * rg + (j & 3);
-        const bool see = slot >= clo && slot < chi;
-        x[j] = see ? (y.there ? x[j] : __builtin_nanf("")) : -INFINITY;
-        if (y.there && slot < any_hi && slot >= any_lo) keep |= 1u << j;
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], u, -ref));
+        l += p;
+        ph[j] = (_Float16)p;
+        if constexpr (TWO) pl[j] = (_Float16)(p - (float)ph[j]);
       }
-      y.v.drop(keep);
-    }
-    float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    if (__ballot(top > ref + 15.f)) {
-      // P' = exp2(x - ref) is kept below 2^15; after a move the maximum of the
-      // column is at 2^7.
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float next = fmaxf(ref, top - 7.f);
-      const float f = __builtin_amdgcn_exp2f(ref - next);
-      ref = next;
-      l *= f;
+      const kvh8 vm = __builtin_bit_cast(kvh8, y.v.m);
+      if constexpr (TWO) om = kv_mfma(vm, pl, om);
+      om = kv_mfma(vm, ph, om);
 #pragma unroll
-      for (int i = 0; i < NT; ++i) o[i] *= f;
-      om *= f;
-    }
-    kvh8 ph, pl;
+      for (int g = 0; g < NG; ++g) {
+        const kvh2 d0 = kv_h2(y.v.d[g][0]), d1 = kv_h2(y.v.d[g][1]), d2 = kv_h2(y.v.d[g][2]), d3 = kv_h2(y.v.d[g][3]);
+        const kvh2 n0 = kv_times(d0, -16.f), n1 = kv_times(d1, -256.f), n2 = kv_times(d2, -16.f), n3 = kv_times(d3, -256.f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float p = __builtin_amdgcn_exp2f(x[j] - ref);
-      l += p;
-      ph[j] = (_Float16)p;
-      if constexpr (TWO) pl[j] = (_Float16)(p - (float)ph[j]);
+        for (int e = 0; e < 2; ++e) {
+          const int i = 2 * g + e;
+          const kvh8 a = kv4_unpack(y.v.w[i >> 2][i & 3], d0, d1, d2, d3, n0, n1, n2, n3);
+          if constexpr (TWO) o[i] = kv_mfma(a, pl, o[i]);
+          o[i] = kv_mfma(a, ph, o[i]);
+        }
+      }
+    };
+    // The page ids, and the first tokens' words, are on their way while the
+    // rows are read.
+    Set xa, xb;
+    ids.fill(s.c, b, t0 >> 6, lane);
+    end = min(any_hi, t0 + ATTN_SEGMENT);
+    load(xa, t0 + 32 * wave);
+    q.load((const T*)s.a.q + (size_t)(sp.r0 + (valid ? row : 0)) * s.a.q_stride + (size_t)head * D, valid, lane, s.a.scale < 0.f ? -1.f : 1.f);
+    // Not negative, so that the largest product is the largest score.
+    unit = q.unit * (fabsf(s.a.scale) * LOG2E);
+    for (int from = t0; from < any_hi; from += ATTN_SEGMENT) {
+      int t = from + 32 * wave;
+      if (from != t0) {
+        ids.fill(s.c, b, from >> 6, lane);
+        end = min(any_hi, from + ATTN_SEGMENT);
+        load(xa, t);
+      }
+      for (; t < end; t += 2 * ATTN_STEP) {
+        load(xb, t + ATTN_STEP);
+        step(xa, t);
+        if (t + ATTN_STEP >= end) break;
+        load(xa, t + 2 * ATTN_STEP);
+        step(xb, t + ATTN_STEP);
+      }
     }
-    const kvh8 vm = __builtin_bit_cast(kvh8, y.v.m);
-    if constexpr (TWO) om = kv_mfma(vm, pl, om);
-    om = kv_mfma(vm, ph, om);
+
+    // The wave's column sums: l over the lane groups, and the minima's part of
+    // dim group g (row g of om) added to its dims.
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      const kvh2 d0 = kv_h2(y.v.d[g][0]), d1 = kv_h2(y.v.d[g][1]), d2 = kv_h2(y.v.d[g][2]), d3 = kv_h2(y.v.d[g][3]);
-      const kvh2 n0 = kv_times(d0, -16.f), n1 = kv_times(d1, -256.f), n2 = kv_times(d2, -16.f), n3 = kv_times(d3, -256.f);
+      const float part = __shfl(om[g & 3], (g >> 2) * 16 + col, 64);
+      o[2 * g] += part;
+      o[2 * g + 1] += part;
+    }
+    // Join the waves, pairs first: the upper of a pair hands over its sums.
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int i = 2 * g + e;
-        const kvh8 a = kv4_unpack(y.v.w[i >> 2][i & 3], d0, d1, d2, d3, n0, n1, n2, n3);
-        if constexpr (TWO) o[i] = kv_mfma(a, pl, o[i]);
-        o[i] = kv_mfma(a, ph, o[i]);
+    for (int half = ATTN_WAVES / 2; half >= 1; half >>= 1) {
+      __syncthreads();
+      if (wave >= half && wave < 2 * half) {
+        const int w = wave - half;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) *reinterpret_cast<kvf4*>(&so[w][col][16 * i + 4 * rg]) = o[i];
+        if (rg == 0) { sr[w][col] = ref; sl[w][col] = l; }
+      }
+      __syncthreads();
+      if (wave < half) {
+        const float r2 = sr[wave][col], next = fmaxf(ref, r2);
+        const float f = __builtin_amdgcn_exp2f(ref - next), f2 = __builtin_amdgcn_exp2f(r2 - next);
+        ref = next;
+        l = l * f + sl[wave][col] * f2;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+          o[i] = o[i] * f + *reinterpret_cast<const kvf4*>(&so[wave][col][16 * i + 4 * rg]) * f2;
       }
     }
-  };
-  Set xa, xb;
-  if (t < any_hi) load(xa, t);
-  for (; t < any_hi; t += 2 * ATTN_STEP) {
-    load(xb, t + ATTN_STEP);
-    step(xa, t);
-    if (t + ATTN_STEP >= any_hi) break;
-    load(xa, t + 2 * ATTN_STEP);
-    step(xb, t + ATTN_STEP);
-  }
-
-  // The wave's column sums: l over the lane groups, and the minima's part of
-  // dim group g (row g of om) added to its dims.
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
+    if (wave != 0 || !valid) continue;
+    if (whole) {
+      const float inv = l != 0.f ? 1.f / l : 0.f;  // NaN stays
+      T* out = (T*)s.a.out + (size_t)(sp.r0 + row) * s.a.out_stride + (size_t)head * D;
 #pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    const float part = __shfl(om[g & 3], (g >> 2) * 16 + col, 64);
-    o[2 * g] += part;
-    o[2 * g + 1] += part;
-  }
-  // Join the waves, pairs first: the upper of a pair hands over its sums.
-#pragma unroll
-  for (int half = ATTN_WAVES / 2; half >= 1; half >>= 1) {
-    __syncthreads();
-    if (wave >= half && wave < 2 * half) {
-      const int w = wave - half;
-#pragma unroll
-      for (int i = 0; i < NT; ++i) *reinterpret_cast<kvf4*>(&so[w][col][16 * i + 4 * rg]) = o[i];
-      if (rg == 0) { sr[w][col] = ref; sl[w][col] = l; }
+      for (int i = 0; i < NT; ++i) {
+        const float y[4] = {o[i][0] * inv, o[i][1] * inv, o[i][2] * inv, o[i][3] * inv};
+        store4(out + 16 * i + 4 * rg, y);
+      }
+      if (s.a.lse && rg == 0)
+        s.a.lse[(size_t)(sp.r0 + row) * s.a.n_heads + head] = l != 0.f ? (ref + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+      continue;
     }
-    __syncthreads();
-    if (wave < half) {
-      const float r2 = sr[wave][col], next = fmaxf(ref, r2);
-      const float f = __builtin_amdgcn_exp2f(ref - next), f2 = __builtin_amdgcn_exp2f(r2 - next);
-      ref = next;
-      l = l * f + sl[wave][col] * f2;
+    AttnPart<D>* part = (AttnPart<D>*)s.a.work + ((size_t)blockIdx.x + b) * gridDim.y + blockIdx.y;
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
-        o[i] = o[i] * f + *reinterpret_cast<const kvf4*>(&so[wave][col][16 * i + 4 * rg]) * f2;
-    }
+    for (int i = 0; i < NT; ++i) *reinterpret_cast<kvf4*>(&part->o[col][16 * i + 4 * rg]) = o[i];
+    if (rg == 0) { part->ref[col] = ref; part->l[col] = l; }
   }
-  if (wave != 0 || !valid) return;
-  if (cut.count == 1) {
-    const float inv = l != 0.f ? 1.f / l : 0.f;  // NaN stays
-    T* out = (T*)s.a.out + (size_t)(sp.r0 + row) * s.a.out_stride + (size_t)head * D;
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const float y[4] = {o[i][0] * inv, o[i][1] * inv, o[i][2] * inv, o[i][3] * inv};
-      store4(out + 16 * i + 4 * rg, y);
-    }
-    if (s.a.lse && rg == 0)
-      s.a.lse[(size_t)(sp.r0 + row) * s.a.n_heads + head] = l != 0.f ? (ref + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
-    return;
-  }
-  AttnPart<D>* part = (AttnPart<D>*)s.a.work + (size_t)blockIdx.x * gridDim.y + blockIdx.y;
-#pragma unroll
-  for (int i = 0; i < NT; ++i) *reinterpret_cast<kvf4*>(&part->o[col][16 * i + 4 * rg]) = o[i];
-  if (rg == 0) { part->ref[col] = ref; part->l[col] = l; }
 }
 
-// Joins the chunks of a sequence: a workgroup per (column of a kv head's
-// tile, sequence).  Each of its waves takes every fourth chunk, 64 lanes over
+// Joins the parts of a sequence: a workgroup per (column of a kv head's
+// tile, sequence).  Each of its waves takes every fourth part, 64 lanes over
 // the dims; LDS adds the four up.
 template <int D, class T>
 __global__ __launch_bounds__(256) void kv4_attn_join(SplitArgs s) {
@@ -314,14 +389,19 @@ __global__ __launch_bounds__(256) void kv4_attn_join(SplitArgs s) {
   const Kv4Span sp = kv4_span(s.rows, b);
   const int ncol = min(16, min(sp.r1 - sp.r0, s.a.max_rows) * s.group - tile * 16);
   if (col >= ncol) return;
-  const int slots = s.c.max_pages * KV4_PAGE;
-  const int chunk = chunk_tokens(s.rows, s.a.window, slots, s.c.n_kv * s.tiles);
-  const int count = chunks_of(s.rows, b, s.a.window, slots, chunk);
+  const int max_slots = s.c.max_pages * KV4_PAGE;
+  Kv4Span own = {0, 0, 0};
+  if (lane < s.rows.n_seq) own = kv4_span(s.rows, lane);
+  const long long share = (axis_total(s.rows, own, s.a.window, max_slots) + s.groups - 1) / s.groups;
+  long long start = lane < b ? rounds_of(own, s.a.window, max_slots) + AXIS_EXTRA : 0;
+  for (int i = 64 + lane; i < b; i += 64) start += rounds_of(kv4_span(s.rows, i), s.a.window, max_slots) + AXIS_EXTRA;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) start += __shfl_xor(start, o, 64);
+  start += AXIS_EXTRA;
+  const long long first = start / share, last = (start + rounds_of(sp, s.a.window, max_slots) - 1) / share;
+  const int count = (int)(last - first) + 1;
   if (count == 1) return;
-  int first = 0;
-  for (int i = lane; i < b; i += 64) first += chunks_of(s.rows, i, s.a.window, slots, chunk);
-  for (int o = 32; o; o >>= 1) first += __shfl_xor(first, o, 64);
-  const AttnPart<D>* part = (const AttnPart<D>*)s.a.work + (size_t)first * gridDim.y + blockIdx.y;
+  const AttnPart<D>* part = (const AttnPart<D>*)s.a.work + (size_t)(first + b) * gridDim.y + blockIdx.y;
   const size_t step = gridDim.y;
   float ref = REF0;
   for (int i = lane; i < count; i += 64) ref = fmaxf(ref, part[i * step].ref[col]);
@@ -350,20 +430,20 @@ __global__ __launch_bounds__(256) void kv4_attn_join(SplitArgs s) {
 }
 
 static int attn_tiles(int group, int max_rows) { return (int)std::min<long long>(65535, ((long long)max_rows * group + 15) / 16); }
-// Chunks of all sequences: their total over the chunk length, which is at
-// least total * per_seq / ATTN_GROUPS, and one more for each sequence.
-static int attn_chunks(int per_seq, int n_seq) { return (ATTN_GROUPS + per_seq - 1) / per_seq + n_seq; }
+// Workgroups that share the axis, of each kv head and column tile.
+template <int D> static int attn_groups(int per_seq) { return std::max(1, ATTN_GROUPS<D> / per_seq); }
 
 size_t kv4_attn_work_bytes(int head_dim, int n_kv, int n_heads, int n_rows, int n_seq, int max_rows, int max_pages) {
-  const int tiles = attn_tiles(n_heads / n_kv, max_rows), per_seq = n_kv * tiles;
-  const size_t part = 16 * (size_t)head_dim * 4 + 128;
-  return std::max<size_t>(256, (size_t)attn_chunks(per_seq, n_seq) * per_seq * part);
+  const int per_seq = n_kv * attn_tiles(n_heads / n_kv, max_rows);
+  const int groups = head_dim == 64 ? attn_groups<64>(per_seq) : head_dim == 128 ? attn_groups<128>(per_seq) : attn_groups<256>(per_seq);
+  return std::max<size_t>(256, ((size_t)groups + n_seq) * per_seq * (16 * (size_t)head_dim * 4 + 128));
 }
 
 template <int D, class T>
-static void attn_go(const SplitArgs& s, hipStream_t st) {
+static void attn_go(SplitArgs s, hipStream_t st) {
   const int per_seq = s.c.n_kv * s.tiles;
-  hipLaunchKernelGGL((kv4_attn_split<D, T>), dim3(attn_chunks(per_seq, s.rows.n_seq), per_seq), dim3(64 * ATTN_WAVES), 0, st, s);
+  s.groups = attn_groups<D>(per_seq);
+  hipLaunchKernelGGL((kv4_attn_split<D, T>), dim3(s.groups, per_seq), dim3(64 * ATTN_WAVES), 0, st, s);
   const int cols = (int)std::min<long long>(16, (long long)s.a.max_rows * s.group);
   hipLaunchKernelGGL((kv4_attn_join<D, T>), dim3(cols, per_seq, s.rows.n_seq), dim3(256), 0, st, s);
 }
@@ -378,7 +458,7 @@ static void attn_typed(int head_dim, const SplitArgs& s, hipStream_t st) {
 hipError_t launch_kv4_attn(int head_dim, const Kv4View& c, int type, const Kv4Rows& rows, const Kv4Attn& a,
                            hipStream_t st) {
   if (kv4_prefill_takes(c, rows, a)) return launch_kv4_prefill(head_dim, c, type, rows, a, st);
-  SplitArgs s{c, rows, a, a.n_heads / c.n_kv, attn_tiles(a.n_heads / c.n_kv, a.max_rows)};
+  SplitArgs s{c, rows, a, a.n_heads / c.n_kv, attn_tiles(a.n_heads / c.n_kv, a.max_rows), 0};
   if (type == ACT_F32) attn_typed<float>(head_dim, s, st);
   else if (type == ACT_F16) attn_typed<_Float16>(head_dim, s, st);
   else attn_typed<bf16_t>(head_dim, s, st);

@@ -54,11 +54,16 @@ struct PageIds {
     base = p;
     ids = p + lane < c.max_pages ? c.table[(size_t)b * c.max_pages + p + lane] : -1;
   }
-  // kv4_block for p >= the base of the first fill, ascending.
-  __device__ __forceinline__ uint8_t* block(const Kv4View& c, int b, int p, int hk, int head_bytes, int lane) {
-    if (p - base >= 64) fill(c, b, p, lane);
+  // kv4_block for base <= p < base + 64.
+  __device__ __forceinline__ uint8_t* at(const Kv4View& c, int p, int hk, int head_bytes) const {
     const int id = __builtin_amdgcn_readlane(ids, p - base);
     return (unsigned)id < (unsigned)c.n_pages ? c.pages + ((size_t)id * c.n_kv + hk) * head_bytes : nullptr;
+  }
+  // The same for ascending p from the first base on.  The refill's wait counts
+  // every load in flight, so loops with loads ahead refill outside.
+  __device__ __forceinline__ uint8_t* block(const Kv4View& c, int b, int p, int hk, int head_bytes, int lane) {
+    if (p - base >= 64) fill(c, b, p, lane);
+    return at(c, p, hk, head_bytes);
   }
 };
 
@@ -149,7 +154,8 @@ template <int D, bool TWO> struct Query {
   static constexpr int NG = D / 32;
   kvh8 hi[NG], lo[TWO ? NG : 1], sums;
   float unit;
-  template <class T> __device__ __forceinline__ void load(const T* row, bool valid, int lane) {
+  // turn: 1, or -1 for a negative scale.
+  template <class T> __device__ __forceinline__ void load(const T* row, bool valid, int lane, float turn = 1.f) {
     const int kg = lane >> 4;
     float x[NG][8], top = 0.f;
     bool finite = true;
@@ -179,7 +185,7 @@ template <int D, bool TWO> struct Query {
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float c = ldexpf(finite ? x[g][j] : 0.f, 10 - e);
+        const float c = ldexpf(finite ? x[g][j] : 0.f, 10 - e) * turn;
         const _Float16 h = (_Float16)c;
         hi[g][j] = h;
         if constexpr (TWO) lo[g][j] = (_Float16)(c - (float)h);
