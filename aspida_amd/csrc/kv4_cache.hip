@@ -9,8 +9,7 @@
 // that head gets d = NaN in every group: key and value read back as NaN, and
 // scores of the slot are NaN, while value scales are always finite (a weight
 // of 0 times them is 0).
-// The arithmetic is exact (f64 differences, remainders by fma): a code never
-// depends on how a quotient was rounded.
+// The arithmetic is exact: a code never depends on how a quotient was rounded.
 #include <algorithm>
 
 #include "kv4.h"
@@ -26,7 +25,7 @@ struct AppendArgs {
   RopeTable t;
 };
 
-struct Kv4Group { float d, m; int q[4]; bool bad; };
+struct Kv4Group { float d, m; int q[8]; bool bad; };
 
 // The spacing of 7-bit steps at d >= 0, a multiple of 2^-24.
 __device__ __forceinline__ float kv4_step_ulp(float d) {
@@ -34,23 +33,37 @@ __device__ __forceinline__ float kv4_step_ulp(float d) {
   return __builtin_bit_cast(float, max(e, (127 - 24) << 23));
 }
 
-// Quantises a group from four values in each of eight neighbouring lanes.
-// Step and codes come from f32 quotients where those leave no doubt and are
-// settled by exact f64 remainders where they might (in f64 throughout, with
-// its divisions, 4097 + 1013 + 2 rows of 8 heads of 128 took 66 us for 18).
-__device__ __forceinline__ Kv4Group kv4_quantise(const float (&x)[4]) {
-  float lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-  int bad = !(__builtin_isfinite(x[0]) && __builtin_isfinite(x[1]) && __builtin_isfinite(x[2]) &&
-              __builtin_isfinite(x[3]));
+// The value of the lane that a row-wise pattern names.
+template <int CTRL> __device__ __forceinline__ float kv4_dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
+
+// Quantises a group from eight values in each of four neighbouring lanes.
+// All in f32 but for the step, and exact all the same.  z = x - m rounded is
+// a multiple of its ulp with an error e of half an ulp at most, and so are
+// the ties (n + 1/2) d (d has 7 bits, 16 d > z): where z is no tie, x - m is
+// on the same side of every tie as z.  The quotient t = z / d, corrected once
+// by its exact remainder, is within 2^-45 before its last rounding: that gives
+// a tie where z is one, and none where z is not, for then z is off by an ulp
+// or more, which is more than half an ulp of t.  So rint(t) is the code, ties
+// to even, unless z is a tie and e decides.
+__device__ __forceinline__ Kv4Group kv4_quantise(const float (&x)[8]) {
+  float lo = x[0], hi = x[0], odd = x[0] * 0.f;  // NaN where a value is not finite
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    lo = fminf(lo, __shfl_xor(lo, o, 64));
-    hi = fmaxf(hi, __shfl_xor(hi, o, 64));
-    bad |= __shfl_xor(bad, o, 64);
+  for (int i = 1; i < 8; ++i) {
+    lo = fminf(lo, x[i]);
+    hi = fmaxf(hi, x[i]);
+    odd = __builtin_fmaf(x[i], 0.f, odd);
   }
+  lo = fminf(lo, kv4_dpp<0xB1>(lo));  // lanes 1 0 3 2
+  hi = fmaxf(hi, kv4_dpp<0xB1>(hi));
+  odd += kv4_dpp<0xB1>(odd);
+  lo = fminf(lo, kv4_dpp<0x4E>(lo));  // 2 3 0 1
+  hi = fmaxf(hi, kv4_dpp<0x4E>(hi));
+  odd += kv4_dpp<0x4E>(odd);
   Kv4Group g;
   g.m = (float)(_Float16)lo;
-  const double m = (double)g.m, z = (double)hi - m;
+  const double z = (double)hi - (double)g.m;
   // A step at or below z / 15, then up while 15 d < z: twice at most, since
   // the quotient is off by less than half a spacing.
   float d = 0.f;
@@ -62,210 +75,207 @@ __device__ __forceinline__ Kv4Group kv4_quantise(const float (&x)[4]) {
     if (15.0 * (double)d < z) d += u;
     if (15.0 * (double)d < z) d += kv4_step_ulp(d);
   }
-  if (bad || !__builtin_isfinite(g.m) || !(d <= KV4_D_MAX)) {
+  if (odd != 0.f || !__builtin_isfinite(g.m) || !(d <= KV4_D_MAX)) {
     g.bad = true;
     g.d = g.m = 0.f;
-    g.q[0] = g.q[1] = g.q[2] = g.q[3] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g.q[i] = 0;
     return g;
   }
   g.bad = false;
   g.d = d;
-  // t is off by less than 16 * 2^-21 where it matters (0 <= t < 16).
   const float inv = d > 0.f ? __builtin_amdgcn_rcpf(d) : 0.f;
-  float n[4];
-  bool close = false;
+  float z8[8], t[8], n[8];
+  bool tie = false;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float t = (x[i] - g.m) * inv;
-    n[i] = __builtin_rintf(t);
-    close |= __builtin_fabsf(t - n[i]) > 0.5f - 0x1p-16f;
+  for (int i = 0; i < 8; ++i) {
+    z8[i] = x[i] - g.m;
+    const float t0 = z8[i] * inv;
+    t[i] = __builtin_fmaf(__builtin_fmaf(-t0, d, z8[i]), inv, t0);
+    n[i] = __builtin_rintf(t[i]);
+    tie |= __builtin_fabsf(t[i] - n[i]) == 0.5f;
   }
-  if (close) {
+  if (tie) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const double rem = __builtin_fma(-(double)n[i], (double)d, (double)x[i] - m), h = 0.5 * (double)d;
-      const bool odd = (int)n[i] & 1;
-      if (rem > h || (rem == h && odd)) n[i] += 1.f;
-      else if (rem < -h || (rem == -h && odd)) n[i] -= 1.f;
+    for (int i = 0; i < 8; ++i) {
+      // x - m = z + e; a tie moves to the side of e.
+      const float back = z8[i] + g.m, e = (x[i] - back) - (g.m - (back - z8[i]));
+      const float to = t[i] + (e > 0.f ? 0.5f : -0.5f);
+      n[i] = e != 0.f && __builtin_fabsf(t[i] - n[i]) == 0.5f ? to : n[i];
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) g.q[i] = (int)fminf(fmaxf(n[i], 0.f), 15.f);
+  for (int i = 0; i < 8; ++i) g.q[i] = (int)__builtin_amdgcn_fmed3f(n[i], 0.f, 15.f);
   return g;
 }
 
-template <class T>
-__device__ __forceinline__ void load4(const T* p, float (&x)[4]) {
-  struct { T v[4]; } r;
-  __builtin_memcpy(&r, p, sizeof(r));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = (float)r.v[i];
+// w with 4-bit code q, not yet in it, at its place j.
+__device__ __forceinline__ uint32_t kv4_put(uint32_t w, uint32_t q, int j) {
+  const int bit = kv4_bit(j);
+  return w | (bit > 28 ? q << bit | q >> (32 - bit) : q << bit);
 }
 
-// One workgroup per (32 slots, kv head, sequence): a block of slots belongs
-// to one workgroup, so the codes of a value dword that this call does not
-// write are kept by a plain read and write of it.  Keys go straight from
-// registers (eight lanes hold a group, two of them a dword); values pass
-// through LDS, since a dword there holds eight tokens.  Every load is issued
-// before the first sum: a decode step, one row a sequence, is one trip to
-// memory behind its lengths and pages (32 sequences 14 -> 9 us).
-template <int D, class T, bool ROPE>
+// One workgroup per (32 slots, sequence) and kv head, or several heads in
+// turn for which the angles are formed once: a block of slots belongs to one
+// workgroup, so the codes of a value dword that this call does not write are
+// kept by a plain read and write of it.  Four lanes hold a group of a token,
+// one key dword each; values pass through LDS, since a dword there holds
+// eight tokens.
+// One loop body serves values and keys, the next group's loads ahead of it
+// (unrolled, 20 KB of code for a few rounds).  Frequencies go through LDS:
+// arguments are far memory, and prompts of 6500 rows in all of 8 heads of 128
+// (bf16) took 57 us with each pair's read from there, 34 now.  Bound by its
+// sums (66% of the issue slots; without the angles 24 us), copies of the same
+// bytes take 7.
+// How keys are rotated: not; values 8 i .. 8 i + 7 with others of that kind
+// (half layout, rot_dim a multiple of 16); in any other way.
+enum : int { ROPE_NONE, ROPE_EIGHTS, ROPE_ANY };
+
+template <int D, class T, int ROPE>
 __global__ __launch_bounds__(256) void kv4_append(AppendArgs a) {
   using L = Kv4L<D>;
   constexpr int NG = L::NG;
-  __shared__ double2 cs[ROPE ? 16 * D / 2 : 1];  // cos, sin [token of the tile][pair]
+  // cos, sin of (pair p, token): 512 bytes a pair, and 64 more every eight
+  // pairs, so that the four lanes of a group read from four parts of the banks.
+  __shared__ double2 cs[ROPE ? 32 * D / 2 + D / 4 : 1];
+  __shared__ double freq[ROPE ? D / 2 : 1];
   __shared__ uint8_t vq[32][D];
   __shared__ int bad[32];  // the token's key or value holds a group that the format does not
-  const int hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const int b = blockIdx.z, tid = threadIdx.x;
   const Kv4Span sp = kv4_span(a.rows, b);
   const int n = sp.r1 - sp.r0, slot0 = sp.len - n;  // the first row's slot, below 0 where kv_len < n
   const int lo = max(slot0, 0), hi = min((long long)sp.len, (long long)a.c.max_pages * KV4_PAGE);
   if (n <= 0 || lo >= hi) return;
   const int half = a.t.rot_dim >> 1;
-  const int c8 = tid & 7;
+  const int kg = tid & 3, t = (tid >> 2) & 31, g0 = tid >> 7;  // groups g0, g0 + 2, ..
+  auto angle = [](int p, int tok) { return 32 * p + 4 * (p >> 3) + tok; };
+  if (ROPE && tid < half) freq[tid] = a.t.freq[tid];
+  __syncthreads();
   for (int blk = (lo >> 5) + blockIdx.x; blk <= (hi - 1) >> 5; blk += gridDim.x) {
-    uint8_t* base = kv4_block(a.c, b, blk >> 1, hk, L::BYTES);
-    if (!base) continue;
+    uint8_t* page = kv4_block(a.c, b, blk >> 1, 0, L::BYTES);
+    if (!page) continue;
     const int s0 = blk << 5, p0 = (blk & 1) * 32;  // first slot, and its token of the page
-    const bool whole = s0 >= lo && s0 + 32 <= hi;
+    const int t0 = max(lo - s0, 0), t1 = min(hi - s0, 32);  // the block's tokens of this call
+    const bool whole = t1 - t0 == 32, in = t >= t0 && t < t1;
     // The nearest row of this call: what a slot of another has is not stored.
-    auto row = [&](int slot) { return (size_t)(sp.r0 + (min(max(slot, lo), hi - 1) - slot0)); };
-    float xv[NG][4], xk[2][NG / 2][4], xo[2][NG / 2][4];
-    int ps[2] = {0, 0};
-    uint32_t old[D / 64];
+    const size_t row = (size_t)(sp.r0 + (s0 + min(max(t, t0), t1 - 1) - slot0));
     if constexpr (ROPE) {
-#pragma unroll
-      for (int tile = 0; tile < 2; ++tile) ps[tile] = a.pos[row(s0 + 16 * tile + (tid >> 4))];
+      // As many threads a pair as the tokens need, in powers of two.
+      const int sh = t1 - t0 > 1 ? 32 - __clz(t1 - t0 - 1) : 0, tok = t0 + (tid & ((1 << sh) - 1));
+      if (tok < t1) {
+        const double at = a.pos[sp.r0 + (s0 + tok - slot0)];
+#pragma unroll 1
+        for (int p = tid >> sh; p < half; p += 256 >> sh) {
+          double s, c;
+          sincos_f64(at * freq[p], s, c);
+          cs[angle(p, tok)] = make_double2(c * a.t.mag, s * a.t.mag);
+        }
+      }
     }
-    {
-      const T* v = (const T*)a.v + row(s0 + (tid >> 3)) * a.vs + (size_t)hk * D + 4 * c8;
+    for (int hk = blockIdx.y; hk < a.c.n_kv; hk += gridDim.y) {
+      uint8_t* base = page + (size_t)hk * L::BYTES;
+      const T* k = (const T*)a.k + row * a.ks + (size_t)hk * D;
+      const T* v = (const T*)a.v + row * a.vs + (size_t)hk * D;
+      struct Values { T x[8]; };
+      // A group's values, and those that its pairs have besides.
+      auto load = [&](int it, Values& x, Values& o) {
+        const bool key = it >= NG / 2;
+        const int d0 = 32 * (g0 + 2 * (key ? it - NG / 2 : it)) + 8 * kg;
+        const T* p = key ? k : v;
+        __builtin_memcpy(&x, p + d0, sizeof(x));
+        if constexpr (ROPE == ROPE_EIGHTS)
+          __builtin_memcpy(&o, p + (d0 < half ? d0 + half : d0 < a.t.rot_dim ? d0 - half : d0), sizeof(o));
+      };
+      uint32_t old[D / 64];
+      uint32_t* word[D / 64];
 #pragma unroll
-      for (int g = 0; g < NG; ++g) load4(v + 32 * g, xv[g]);
-    }
+      for (int c = 0; c < D / 64; ++c) {  // value dword (lane group rg, dim d)
+        const int i = tid + 256 * c, rg = i / D, d = i % D;
+        word[c] = reinterpret_cast<uint32_t*>(base + L::value_word(p0 + 4 * rg, d));
+        old[c] = *word[c];
+      }
+      Values x, o;
+      load(0, x, o);
+      if (tid < 32) bad[tid] = 0;
+      __syncthreads();
+#pragma unroll 1
+      for (int it = 0; it < NG; ++it) {
+        Values nx, no;
+        load(min(it + 1, NG - 1), nx, no);
+        const bool key = it >= NG / 2;
+        const int g = g0 + 2 * (key ? it - NG / 2 : it), d0 = 32 * g + 8 * kg;
+        float y[8];
 #pragma unroll
-    for (int tile = 0; tile < 2; ++tile) {
-      const T* k = (const T*)a.k + row(s0 + 16 * tile + ((tid >> 3) & 15)) * a.ks + (size_t)hk * D;
+        for (int e = 0; e < 8; ++e) y[e] = (float)x.x[e];
+        // (a c - b s, a s + b c), rounded to f32 once.
+        if constexpr (ROPE == ROPE_EIGHTS) {
+          if (key && d0 < a.t.rot_dim) {
+            const bool second = d0 >= half;
+            const double2* w = cs + angle(second ? d0 - half : d0, t);
 #pragma unroll
-      for (int it = 0; it < NG / 2; ++it) {
-        const int d0 = 32 * (2 * it + (tid >> 7)) + 4 * c8;
-        load4(k + d0, xk[tile][it]);
-        if constexpr (ROPE) {
-          // The other halves of the four pairs.
-          auto other = [&](int d) { return d < half ? d + half : d < a.t.rot_dim ? d - half : d; };
-          if (a.t.interleaved) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) xo[tile][it][e] = xk[tile][it][e ^ 1];
-          } else if (!(half & 3)) {
-            load4(k + other(d0), xo[tile][it]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) xo[tile][it][e] = (float)k[other(d0 + e)];
+            for (int e = 0; e < 8; ++e) {
+              const float ot = o.x[e];
+              y[e] = (float)__builtin_fma((double)(second ? ot : -ot), w[32 * e].y, (double)y[e] * w[32 * e].x);
+            }
           }
-        }
-      }
-    }
-    uint32_t* vw[D / 64];
+        } else if constexpr (ROPE == ROPE_ANY) {
+          if (key) {
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) {
-      const int i = tid + 256 * c, rg = i / D, d = i - rg * D;
-      vw[c] = reinterpret_cast<uint32_t*>(base + L::value_word(p0 + 4 * rg, d));
-      old[c] = 0;
-      if (!whole) old[c] = *vw[c];
-    }
-    if (tid < 32) bad[tid] = 0;
-    __syncthreads();
-    {
-      const int t = tid >> 3, slot = s0 + t;
-      const bool in = slot >= lo && slot < hi;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const Kv4Group q = kv4_quantise(xv[g]);
-        *reinterpret_cast<uint32_t*>(&vq[t][32 * g + 4 * c8]) =
-            (uint32_t)q.q[0] | (uint32_t)q.q[1] << 8 | (uint32_t)q.q[2] << 16 | (uint32_t)q.q[3] << 24;
-        if (in && c8 == 0) {
-          if (q.bad) bad[t] = 1;
-          *reinterpret_cast<_Float16*>(base + L::value_d(p0 + t, g)) = (_Float16)q.d;
-          *reinterpret_cast<_Float16*>(base + L::value_m(p0 + t, g)) = (_Float16)q.m;
-        }
-      }
-    }
-#pragma unroll
-    for (int tile = 0; tile < 2; ++tile) {
-      const int f = s0 + 16 * tile;
-      if (f >= hi || f + 16 <= lo) continue;
-      if constexpr (ROPE) {
-        __syncthreads();
-        if (f + (tid >> 4) >= lo && f + (tid >> 4) < hi) {
-          for (int p = tid & 15; p < half; p += 16) {
-            double s, c;
-            sincos_f64((double)ps[tile] * a.t.freq[p], s, c);
-            cs[(tid >> 4) * half + p] = make_double2(c * a.t.mag, s * a.t.mag);
-          }
-        }
-        __syncthreads();
-      }
-      const int t = (tid >> 3) & 15, slot = f + t, tok = p0 + 16 * tile + t;
-      const bool in = slot >= lo && slot < hi;
-#pragma unroll
-      for (int it = 0; it < NG / 2; ++it) {
-        const int g = 2 * it + (tid >> 7), d0 = 32 * g + 4 * c8;
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = xk[tile][it][e];
-        if constexpr (ROPE) {
-          if (in) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 8; ++e) {
               const int d = d0 + e;
-              if (d < a.t.rot_dim) {
-                const bool second = a.t.interleaved ? (d & 1) : d >= half;
-                const int p = a.t.interleaved ? d >> 1 : second ? d - half : d;
-                const double2 w = cs[t * half + p];
-                const double me = xk[tile][it][e], o = xo[tile][it][e];
-                // (a c - b s, a s + b c), rounded to f32 once.
-                x[e] = (float)(second ? __builtin_fma(o, w.y, me * w.x) : __builtin_fma(me, w.x, -(o * w.y)));
-              }
+              if (d >= a.t.rot_dim) continue;
+              const bool second = a.t.interleaved ? (d & 1) : d >= half;
+              const double2 w = cs[angle(a.t.interleaved ? d >> 1 : second ? d - half : d, t)];
+              const float ot = a.t.interleaved ? (float)x.x[e ^ 1] : (float)k[second ? d - half : d + half];
+              y[e] = (float)__builtin_fma((double)(second ? ot : -ot), w.y, (double)y[e] * w.x);
             }
           }
         }
-        const Kv4Group q = kv4_quantise(x);
+        const Kv4Group q = kv4_quantise(y);
+        if (key) {
+          uint32_t w = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w = kv4_put(w, (uint32_t)q.q[e], e);
+          if (in) *reinterpret_cast<uint32_t*>(base + L::key_word(p0 + t, g, kg)) = w;
+        } else {
+          kvu2 w = {0, 0};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e >> 2] |= (uint32_t)q.q[e] << (8 * (e & 3));
+          *reinterpret_cast<kvu2*>(&vq[t][32 * g + 8 * kg]) = w;
+        }
+        if (in && kg == 0) {
+          if (q.bad) bad[t] = 1;
+          const int d = key ? L::key_d(p0 + t, g) : L::value_d(p0 + t, g);
+          *reinterpret_cast<_Float16*>(base + d) = (_Float16)q.d;
+          *reinterpret_cast<_Float16*>(base + d + (key ? 2 * NG : 64 * NG)) = (_Float16)q.m;
+        }
+        x = nx;
+        o = no;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        const int i = tid + 256 * c, rg = i / D, d = i % D;
         uint32_t w = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t left = (c8 & 1) ? kv4_bit(4 + e) : kv4_bit(e);
-          w |= __builtin_amdgcn_alignbit((uint32_t)q.q[e], (uint32_t)q.q[e], 32 - left);
+        for (int j = 0; j < 8; ++j) w = kv4_put(w, vq[16 * (j >> 2) + 4 * rg + (j & 3)][d], j);
+        if (!whole) {
+          uint32_t mine = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int u = 16 * (j >> 2) + 4 * rg + (j & 3);
+            if (u >= t0 && u < t1) mine = kv4_put(mine, 15u, j);
+          }
+          w = (w & mine) | (old[c] & ~mine);
         }
-        w |= (uint32_t)__shfl_xor((int)w, 1, 64);
-        if (in && !(c8 & 1)) *reinterpret_cast<uint32_t*>(base + L::key_word(tok, g, c8 >> 1)) = w;
-        if (in && c8 == 0) {
-          if (q.bad) bad[16 * tile + t] = 1;
-          *reinterpret_cast<_Float16*>(base + L::key_d(tok, g)) = (_Float16)q.d;
-          *reinterpret_cast<_Float16*>(base + L::key_m(tok, g)) = (_Float16)q.m;
-        }
+        *word[c] = w;
       }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < D / 64; ++c) {
-      const int i = tid + 256 * c, rg = i / D, d = i - rg * D;
-      uint32_t w = 0, mine = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int t = 16 * (j >> 2) + 4 * rg + (j & 3), slot = s0 + t;
-        if (slot >= lo && slot < hi) {
-          const uint32_t code = vq[t][d];
-          w |= __builtin_amdgcn_alignbit(code, code, (uint32_t)((32 - kv4_bit(j)) & 31));
-          mine |= __builtin_amdgcn_alignbit(15u, 15u, (uint32_t)((32 - kv4_bit(j)) & 31));
-        }
+      // (A slot that is not this call's has no flag.)
+      if (tid < 32 && bad[tid]) {
+        for (int g = 0; g < NG; ++g) *reinterpret_cast<uint16_t*>(base + L::key_d(p0 + tid, g)) = 0x7E00;
       }
-      if (mine) *vw[c] = (old[c] & ~mine) | w;
+      __syncthreads();
     }
-    // (A slot that is not this call's has no flag.)
-    if (tid < 32 && bad[tid]) {
-#pragma unroll
-      for (int g = 0; g < NG; ++g) *reinterpret_cast<uint16_t*>(base + L::key_d(p0 + tid, g)) = 0x7E00;
-    }
-    __syncthreads();
   }
 }
 
@@ -338,16 +348,26 @@ __global__ __launch_bounds__(256) void kv4_read(ReadArgs a) {
 }
 
 // Workgroups per (kv head, sequence): one for every 32-slot block of an
-// average sequence; longer ones take theirs in turns.
-static unsigned blocks_of(const Kv4Rows& r) {
-  return (unsigned)std::min<long long>(65535, ((long long)r.n_rows + r.n_seq - 1) / r.n_seq / 32 + 2);
+// average sequence, and up to 4096 in all for longer ones, which otherwise take
+// theirs in turns (prompts of 4097, 1013 and 2 rows: 57 us with 55 of 128
+// blocks at a time).
+static unsigned blocks_of(const Kv4Rows& r, int n_kv) {
+  const long long most = r.n_rows / 32 + 2, mean = ((long long)r.n_rows + r.n_seq - 1) / r.n_seq / 32 + 2;
+  const long long room = 4096 / ((long long)n_kv * r.n_seq);
+  return (unsigned)std::min<long long>(65535, std::min(most, std::max(mean, room)));
 }
 
 template <int D, class T>
 static void append_go(const AppendArgs& a, bool rope, hipStream_t s) {
-  const dim3 grid(blocks_of(a.rows), a.c.n_kv, a.rows.n_seq);
-  if (rope) hipLaunchKernelGGL((kv4_append<D, T, true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((kv4_append<D, T, false>), grid, dim3(256), 0, s, a);
+  const unsigned blocks = blocks_of(a.rows, a.c.n_kv);
+  // Heads a workgroup takes in turn, as far as that leaves three workgroups a
+  // compute unit (6500 rows of 8 heads: one 34.7 us, two 33.8, four 65, by a form before this).
+  const long long all = ((long long)a.rows.n_rows / 32 + a.rows.n_seq) * a.c.n_kv;
+  const int turns = rope ? (int)std::min<long long>(std::max<long long>(all / 768, 1), a.c.n_kv) : 1;
+  const dim3 grid(blocks, (a.c.n_kv + turns - 1) / turns, a.rows.n_seq);
+  if (!rope) hipLaunchKernelGGL((kv4_append<D, T, ROPE_NONE>), grid, dim3(256), 0, s, a);
+  else if (a.t.interleaved || a.t.rot_dim % 16) hipLaunchKernelGGL((kv4_append<D, T, ROPE_ANY>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((kv4_append<D, T, ROPE_EIGHTS>), grid, dim3(256), 0, s, a);
 }
 template <int D>
 static void append_typed(const AppendArgs& a, int type, bool rope, hipStream_t s) {
@@ -376,7 +396,7 @@ hipError_t launch_kv4_append(int head_dim, const Kv4View& c, int type, const voi
 
 template <int D>
 static void read_typed(const ReadArgs& a, int type, hipStream_t s) {
-  const dim3 grid(blocks_of(a.rows), a.c.n_kv, a.rows.n_seq);
+  const dim3 grid(blocks_of(a.rows, a.c.n_kv), a.c.n_kv, a.rows.n_seq);
   if (type == ACT_F32) hipLaunchKernelGGL((kv4_read<D, float>), grid, dim3(256), 0, s, a);
   else if (type == ACT_F16) hipLaunchKernelGGL((kv4_read<D, _Float16>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((kv4_read<D, bf16_t>), grid, dim3(256), 0, s, a);

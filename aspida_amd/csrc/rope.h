@@ -6,6 +6,7 @@
 // an f32 angle is off by a hundredth of a radian.
 #pragma once
 #include <hip/hip_runtime.h>
+#include <stdint.h>
 
 namespace kq {
 
@@ -37,7 +38,9 @@ template <class T> __device__ __forceinline__ float act_f32(T v) { return (float
 // n times what a third would add is below 2^-70), then the Taylor series at
 // |r| <= pi/4, whose first dropped terms are r^19/19! and r^18/18! (< 2^-58).
 __device__ __forceinline__ void sincos_f64(double theta, double& s, double& c) {
-  const double n = __builtin_rint(theta * 0.63661977236758134308);
+  // n + 1.5 2^52 has n's low bits at the end of its significand.
+  const double at = __builtin_fma(theta, 0.63661977236758134308, 6755399441055744.0);
+  const double n = at - 6755399441055744.0;
   double r = __builtin_fma(-n, 1.5707963267948965580, theta);
   r = __builtin_fma(-n, 6.1232339957367660359e-17, r);
   const double z = r * r;
@@ -59,7 +62,7 @@ __device__ __forceinline__ void sincos_f64(double theta, double& s, double& c) {
   q = __builtin_fma(q, z, 1.0 / 24.0);
   q = __builtin_fma(q, z, -0.5);
   const double cs = __builtin_fma(q, z, 1.0);
-  const int k = (int)(long long)n & 3;
+  const int k = (int)__builtin_bit_cast(uint64_t, at) & 3;
   const double u = (k & 1) ? cs : sn, w = (k & 1) ? sn : cs;
   s = (k & 2) ? -u : u;
   c = (k == 1 || k == 2) ? -w : w;
