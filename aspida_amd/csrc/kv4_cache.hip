@@ -361,7 +361,7 @@ template <int D, class T>
 static void append_go(const AppendArgs& a, bool rope, hipStream_t s) {
   const unsigned blocks = blocks_of(a.rows, a.c.n_kv);
   // Heads a workgroup takes in turn, as far as that leaves three workgroups a
-  // compute unit (6500 rows of 8 heads: one 34.7 us, two 33.8, four 65, by a form before this).
+  // compute unit (6500 rows of 8 heads: one 34.7 us, two 33.8).
   const long long all = ((long long)a.rows.n_rows / 32 + a.rows.n_seq) * a.c.n_kv;
   const int turns = rope ? (int)std::min<long long>(std::max<long long>(all / 768, 1), a.c.n_kv) : 1;
   const dim3 grid(blocks, (a.c.n_kv + turns - 1) / turns, a.rows.n_seq);

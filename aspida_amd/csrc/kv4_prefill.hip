@@ -473,12 +473,18 @@ static hipError_t prefill_typed(int head_dim, const PrefillArgs& s, hipStream_t 
   return prefill_go<256, T, 4>(s, st);
 }
 
-// Many rows: enough columns to fill the 32 of a wave several times over, and
-// workgroups for most of the card (the split kernel cuts the slots instead).
+// The host knows rows, not lengths.  A workgroup here walks all slots of 256
+// columns; the split kernel (kv4_attn.hip) cuts the slots, and reads them once
+// per 16 columns.  So this one is for sequences of many columns, and for
+// enough of them in all that most compute units have some:
+//   columns of a (sequence, kv head), card full (64 sequences of 3000 slots,
+//   32/8 heads, bf16): 48 here 241 us, split 194; 64: 243 and 223; 96: 246
+//   and 372 (f32 96: 389 and 409; heads of 256 48: 201 and 194);
+//   rows x heads in all (20000 slots, bf16): 12288 here 679 us, split 400;
+//   24576: 681 and 787 (f32 1066 and 925; heads of 256 12288: 1133 and 813).
 bool kv4_prefill_takes(const Kv4View& c, const Kv4Rows& rows, const Kv4Attn& a) {
   const long long cols = (long long)std::min(a.max_rows, rows.n_rows) * (a.n_heads / c.n_kv);
-  const long long tiles = (cols + 255) / 256;
-  return cols >= 96 && tiles <= 65535 && tiles * c.n_kv * rows.n_seq >= 1;
+  return cols >= 80 && (cols + 255) / 256 <= 65535 && (long long)rows.n_rows * a.n_heads >= 20480;
 }
 
 hipError_t launch_kv4_prefill(int head_dim, const Kv4View& c, int type, const Kv4Rows& rows, const Kv4Attn& a,

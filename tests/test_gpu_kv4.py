@@ -327,8 +327,17 @@ def _bounds(ty, n, pv, sk, out, lse):
     return b_out, b_lse
 
 
-def _attend(c, ty, q, starts, lens, heads, scale, window=0, max_rows=None, want_lse=True, out_stride=None):
+def _attend(c, ty, q, starts, lens, heads, scale, window=0, max_rows=None, want_lse=True, out_stride=None, many=False):
+    """many: in a batch of at least 80 columns a sequence and 20480 in all, most
+    of them rows behind the last sequence, as the kernel for many rows takes."""
     torch = torch_cuda()
+    if many:
+        n = q.shape[0]
+        q = torch.cat([q, q.new_zeros((max(80, -(-20480 // heads)), q.shape[1]))])
+        out, lse = _attend(c, ty, q, starts, lens, heads, scale, window, max(80, max_rows or int(np.diff(starts).max())),
+                           want_lse, out_stride)
+        assert (out[n:] == 7).all() and (lse[n:] == 7).all()
+        return out[:n], lse[:n]
     n, dim = q.shape[0], c.dim
     rows = np.diff(starts)
     st, ln = _i32(starts), _i32(lens)
@@ -397,20 +406,46 @@ ATTENTION = [
 
 @pytest.mark.parametrize("ty", [aa.F32, aa.BF16, aa.F16], ids=NAMES.get)
 @pytest.mark.parametrize("case", ATTENTION, ids=lambda c: f"d{c[0]}h{c[1]}k{c[2]}r{'_'.join(map(str, c[3]))}n{'_'.join(map(str, c[4]))}w{c[5]}")
-def test_attention(case, ty):
+@pytest.mark.parametrize("many", [False, True], ids=["few", "many"])
+def test_attention(case, ty, many):
     dim, heads, kv, rows, lens, window = case
     gen = np.random.default_rng(dim + heads + sum(lens))
     c = _filled(gen, dim, kv, lens, max_pages=-(-max(lens) // 64) + 1)
     st = _starts(rows)
     q = _dev(2 * gen.standard_normal((st[-1], heads * dim)).astype(np.float32), ty)
-    out, lse = _attend(c, ty, q, st, lens, heads, dim ** -0.5, window)
+    out, lse = _attend(c, ty, q, st, lens, heads, dim ** -0.5, window, many=many)
     _check(c, ty, q, st, lens, heads, dim ** -0.5, window, out, lse)
-    again, lse2 = _attend(c, ty, q, st, lens, heads, dim ** -0.5, window, max_rows=max(1, max(rows)))
+    again, lse2 = _attend(c, ty, q, st, lens, heads, dim ** -0.5, window, max_rows=max(1, max(rows)), many=many)
     assert (again == out).all() and (lse2 == lse).all()
 
 
-@pytest.mark.parametrize("rows,lens", [([1, 1], [200, 40]), ([40, 3], [100, 40])], ids=["decode", "prompt"])
-def test_attention_strides_types_of_rows_and_untouched_memory(rows, lens):
+# dim, heads, kv, rows, lens, window: shares of a long axis, a sequence in
+# parts of several workgroups and several sequences in one, over 64 of them.
+SHARES = [
+    (64, 4, 1, [1], [9001], 0),
+    (64, 4, 2, [3, 1], [4100, 33], 2000),
+    (256, 2, 1, [1, 1], [5000, 1], 0),
+    (128, 4, 4, [5], [3300], 0),
+    (64, 2, 1, [1, 2, 0] * 30, [(37 * i) % 300 for i in range(90)], 0),
+    (128, 8, 1, [1] * 129, [2000 if i == 70 else i % 7 for i in range(129)], 50),
+]
+
+
+@pytest.mark.parametrize("ty", [aa.F32, aa.BF16], ids=NAMES.get)
+@pytest.mark.parametrize("case", SHARES, ids=lambda c: f"d{c[0]}h{c[1]}k{c[2]}s{len(c[3])}n{max(c[4])}w{c[5]}")
+def test_attention_shares_and_parts(case, ty):
+    dim, heads, kv, rows, lens, window = case
+    gen = np.random.default_rng(dim + len(rows))
+    c = _filled(gen, dim, kv, lens, max_pages=-(-max(lens) // 64))
+    st = _starts(rows)
+    q = _dev(2 * gen.standard_normal((st[-1], heads * dim)).astype(np.float32), ty)
+    out, lse = _attend(c, ty, q, st, lens, heads, dim ** -0.5, window)
+    _check(c, ty, q, st, lens, heads, dim ** -0.5, window, out, lse)
+
+
+@pytest.mark.parametrize("rows,lens,many", [([1, 1], [200, 40], False), ([40, 3], [100, 40], False),
+                                            ([100, 3], [130, 40], True)], ids=["decode", "prompt", "many"])
+def test_attention_strides_types_of_rows_and_untouched_memory(rows, lens, many):
     """Rows at odd strides, rows behind the last sequence, max_rows that is not
     the longest, and no lse wanted."""
     torch = torch_cuda()
@@ -421,24 +456,24 @@ def test_attention_strides_types_of_rows_and_untouched_memory(rows, lens):
         st = _starts(rows)
         wide = heads * dim + 3
         q = _dev(gen.standard_normal((st[-1] + 2, wide)).astype(np.float32), ty)
-        out, lse = _attend(c, ty, q, st, lens, heads, 0.2, out_stride=wide)
+        out, lse = _attend(c, ty, q, st, lens, heads, 0.2, out_stride=wide, many=many)
         n = int(st[-1])
         assert (out[n:] == 7).all() and (out[:, heads * dim:] == 7).all() and (lse[n:] == 7).all()
         _check(c, ty, q, st, lens, heads, 0.2, 0, out, lse)
         for mr in (1, 17, 1000):
-            o2, l2 = _attend(c, ty, q, st, lens, heads, 0.2, max_rows=mr, out_stride=wide)
+            o2, l2 = _attend(c, ty, q, st, lens, heads, 0.2, max_rows=mr, out_stride=wide, many=many)
             for b, r in enumerate(rows):  # rows past max_rows: NaN
-                over = slice(int(st[b]) + min(r, mr), int(st[b + 1]))
+                over = slice(int(st[b]) + min(r, max(mr, 80) if many else mr), int(st[b + 1]))
                 assert torch.isnan(o2[over, :heads * dim]).all() and torch.isnan(l2[over]).all()
                 o2[over], l2[over] = out[over], lse[over]
             _check(c, ty, q, st, lens, heads, 0.2, 0, o2, l2)
-        o3, l3 = _attend(c, ty, q, st, lens, heads, 0.2, out_stride=wide, want_lse=False)
+        o3, l3 = _attend(c, ty, q, st, lens, heads, 0.2, out_stride=wide, want_lse=False, many=many)
         assert (o3 == out).all() and (l3 == 7).all()
 
 
-@pytest.mark.parametrize("rows", [1, 40], ids=["decode", "prompt"])
+@pytest.mark.parametrize("rows,many", [(1, False), (40, False), (40, True)], ids=["decode", "prompt", "many"])
 @pytest.mark.parametrize("ty", [aa.F32, aa.F16], ids=NAMES.get)
-def test_attention_scales_of_the_values(rows, ty):
+def test_attention_scales_of_the_values(rows, many, ty):
     """One-hot and flat softmaxes, tiny and large keys and values, zero queries,
     constant keys, a slot whose weight dwarfs the others' with values near 0."""
     gen = np.random.default_rng(31)
@@ -452,13 +487,13 @@ def test_attention_scales_of_the_values(rows, ty):
         v[0] *= np.float32(1e-3)
         c.append(aa.F32, _dev(k), _dev(v), [0, n], [n])
         q = _dev((qq * gen.standard_normal((rows, heads * dim))).astype(np.float32), ty)
-        out, lse = _attend(c, ty, q, [0, rows], [n], heads, scale)
+        out, lse = _attend(c, ty, q, [0, rows], [n], heads, scale, many=many)
         _check(c, ty, q, [0, rows], [n], heads, scale, 0, out, lse)
 
 
-@pytest.mark.parametrize("rows", [1, 40], ids=["decode", "prompt"])
+@pytest.mark.parametrize("rows,many", [(1, False), (40, False), (40, True)], ids=["decode", "prompt", "many"])
 @pytest.mark.parametrize("ty", [aa.F32, aa.BF16], ids=NAMES.get)
-def test_masked_slots_never_matter_and_seen_ones_always(rows, ty):
+def test_masked_slots_never_matter_and_seen_ones_always(rows, many, ty):
     """Slots behind the length and before the window hold NaN scales; a NaN or
     infinity in a query, a NaN key in sight and a page that is not there make
     the rows that see them NaN, and no others."""
@@ -473,16 +508,16 @@ def test_masked_slots_never_matter_and_seen_ones_always(rows, ty):
     host = gen.standard_normal((2 * rows, heads * dim)).astype(np.float32)
     q = _dev(host, ty)
     # Every row of sequence 0 sees slots 61 and up at least, none below 30.
-    out, lse = _attend(c, ty, q, st, lens, heads, 0.1, window=60)
+    out, lse = _attend(c, ty, q, st, lens, heads, 0.1, window=60, many=many)
     _check(c, ty, q, st, lens, heads, 0.1, 60, out, lse, kvs)
-    out, lse = _attend(c, ty, q, st, lens, heads, 0.1)
+    out, lse = _attend(c, ty, q, st, lens, heads, 0.1, many=many)
     assert np.isnan(_host(out)[:rows]).all() and np.isnan(_host(lse)[:rows]).all()
     assert np.isfinite(_host(out)[rows:]).all()
     host2 = host.copy()
     host2[0, 3] = np.nan
     host2[rows, dim + 5] = np.inf
     q2 = _dev(host2, ty)
-    out, lse = _attend(c, ty, q2, st, lens, heads, 0.1, window=60)
+    out, lse = _attend(c, ty, q2, st, lens, heads, 0.1, window=60, many=many)
     o = _host(out).reshape(2 * rows, heads, dim)
     assert np.isnan(o[0, 0]).all() and np.isnan(o[rows, 1]).all()
     o[0, 0], o[rows, 1] = 0, 0
@@ -491,11 +526,11 @@ def test_masked_slots_never_matter_and_seen_ones_always(rows, ty):
         table = c.host_table.copy()
         table[1, 0] = page
         c.set_table(table)
-        out, lse = _attend(c, ty, q, st, lens, heads, 0.1, window=60)
+        out, lse = _attend(c, ty, q, st, lens, heads, 0.1, window=60, many=many)
         assert np.isnan(_host(out)[rows:]).all() and np.isfinite(_host(out)[:rows]).all()
     c.set_table(c.host_table)
     long = [4 * 64 + rows + 70, lens[1]]  # longer than the table: its rows see slots past it
-    out, _ = _attend(c, ty, q, st, long, heads, 0.1, window=60)
+    out, _ = _attend(c, ty, q, st, long, heads, 0.1, window=60, many=many)
     assert np.isnan(_host(out)[:rows]).all() and np.isfinite(_host(out)[rows:]).all()
 
 
