@@ -3,6 +3,7 @@
 // can see are checked here; lengths, row starts and page ids live on the
 // device and are bounded by the kernels.
 #include <cerrno>
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <new>
@@ -48,6 +49,9 @@ int rows_of(int n_rows, int n_seq, const int* row_start, const int* kv_len, kq::
 bool valid_rows(const void* p, int type, long long stride, int heads, int head_dim) {
   return type_bytes(type) && aligned(p, (size_t)type_bytes(type)) && stride >= (long long)heads * head_dim;
 }
+
+// The bound on a sequence's rows that grids are cut for: never above all rows.
+int longest(int max_rows, int n_rows) { return std::min(max_rows, std::max(n_rows, 1)); }
 
 bool valid_heads(const aspida_kv4* c, int n_heads) {
   return n_heads >= 1 && n_heads <= 65535 && n_heads % c->n_kv == 0;
@@ -178,8 +182,7 @@ extern "C" long long aspida_kv4_attn_work_bytes(const aspida_kv4* cache, int n_h
                                                 int max_rows) {
   if (!valid_cache(cache) || !valid_heads(cache, n_heads) || n_rows < 0 || n_seq < 0 || n_seq > 65535 || max_rows < 1)
     return -EINVAL;
-  return (long long)kq::kv4_attn_work_bytes(cache->head_dim, cache->n_kv, n_heads, n_rows, n_seq, max_rows,
-                                            cache->max_pages);
+  return (long long)kq::kv4_attn_work_bytes(cache->head_dim, cache->n_kv, n_heads, n_seq, longest(max_rows, n_rows));
 }
 
 extern "C" int aspida_kv4_attn_dev(const aspida_kv4* cache, int type, const void* q, long long q_stride, int n_heads,
@@ -194,7 +197,7 @@ extern "C" int aspida_kv4_attn_dev(const aspida_kv4* cache, int type, const void
       !valid_rows(out, type, out_stride, n_heads, cache->head_dim) || (lse && !aligned(lse, 4)) ||
       !aligned(work, 256))
     return -EINVAL;
-  kq::Kv4Attn a{q, q_stride, out, out_stride, lse, work, n_heads, max_rows, window, scale};
+  kq::Kv4Attn a{q, q_stride, out, out_stride, lse, work, n_heads, longest(max_rows, n_rows), window, scale};
   return done(kq::launch_kv4_attn(cache->head_dim, view(cache), type, r, a, (hipStream_t)stream),
               "aspida_kv4_attn_dev");
 }
@@ -210,7 +213,7 @@ extern "C" int aspida_kv4_weigh_dev(const aspida_kv4* cache, int type, const voi
   if (!valid_rows(q, type, q_stride, n_heads, cache->head_dim) || !aligned(lse, 4) ||
       (acc_in && !aligned(acc_in, 4)) || !aligned(acc_out, 4) || acc_stride < 1)
     return -EINVAL;
-  kq::Kv4Weigh w{q, q_stride, lse, acc_in, acc_out, acc_stride, n_heads, max_rows, window, scale};
+  kq::Kv4Weigh w{q, q_stride, lse, acc_in, acc_out, acc_stride, n_heads, longest(max_rows, n_rows), window, scale};
   return done(kq::launch_kv4_weigh(cache->head_dim, view(cache), type, r, w, (hipStream_t)stream),
               "aspida_kv4_weigh_dev");
 }

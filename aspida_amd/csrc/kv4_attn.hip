@@ -21,6 +21,11 @@
 // workgroup takes what of one sequence or of several lies in its share, and a
 // second launch joins the parts of a sequence.  All of it follows from the
 // lengths on the device, which the host does not know.
+// Bound by the vector units: a wave's round of 32 tokens is about 300 of their
+// instructions (unpacking, exp2, the two planes of P) in 1800 cycles, with
+// two waves a SIMD, and 45 matrix instructions beside them.  130001 slots of 8
+// kv heads of 128 (f32, 166 MB) take 42 us, 4.0 TB/s, of 32 at the rate of a
+// large copy; 64 lanes of up to 8192 slots (bf16, 330 MB) 79 us, 4.2 TB/s.
 #include <algorithm>
 
 #include "kv4_mma.h"
@@ -32,9 +37,8 @@ constexpr int ATTN_STEP = 32 * ATTN_WAVES;  // tokens of a workgroup's round
 // Tokens whose page ids a wave holds at once: whole rounds, within 64 pages
 // wherever in a page they start.
 constexpr int ATTN_SEGMENT = (4096 - 32) / ATTN_STEP * ATTN_STEP;
-// Workgroups that the chunks are cut for: three for each of 256 CUs.
-// Workgroups that fit at once: 256 CUs times what their registers allow (134,
-// 198 and over 256 for heads of 64, 128 and 256).  One round of equal shares
+// Workgroups that fit at once: 256 CUs times what their registers allow (under
+// 168, 256 and 512 for heads of 64, 128 and 256).  One round of equal shares
 // measured against 1.5 and 2 rounds (32/8 heads, f32): 130001 slots 47, 59
 // and 57 us; 16 lanes of 8000 45, 56 and 54 us.
 template <int D> constexpr int ATTN_GROUPS = D == 64 ? 768 : D == 128 ? 512 : 256;
@@ -291,7 +295,8 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, D == 64 ? 3 : D == 128 ? 2 : 1) vo
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         const kvh2 d0 = kv_h2(y.v.d[g][0]), d1 = kv_h2(y.v.d[g][1]), d2 = kv_h2(y.v.d[g][2]), d3 = kv_h2(y.v.d[g][3]);
-        const kvh2 n0 = kv_times(d0, -16.f), n1 = kv_times(d1, -256.f), n2 = kv_times(d2, -16.f), n3 = kv_times(d3, -256.f);
+        const kvh2 n0 = kv_times(d0, -16.f), n1 = kv_times(d1, -256.f);
+        const kvh2 n2 = kv_times(d2, -16.f), n3 = kv_times(d3, -256.f);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int i = 2 * g + e;
@@ -307,7 +312,8 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, D == 64 ? 3 : D == 128 ? 2 : 1) vo
     ids.fill(s.c, b, t0 >> 6, lane);
     end = min(any_hi, t0 + ATTN_SEGMENT);
     load(xa, t0 + 32 * wave);
-    q.load((const T*)s.a.q + (size_t)(sp.r0 + (valid ? row : 0)) * s.a.q_stride + (size_t)head * D, valid, lane, s.a.scale < 0.f ? -1.f : 1.f);
+    q.load((const T*)s.a.q + (size_t)(sp.r0 + (valid ? row : 0)) * s.a.q_stride + (size_t)head * D, valid, lane,
+           s.a.scale < 0.f ? -1.f : 1.f);
     // Not negative, so that the largest product is the largest score.
     unit = q.unit * (fabsf(s.a.scale) * LOG2E);
     for (int from = t0; from < any_hi; from += ATTN_SEGMENT) {
@@ -429,13 +435,18 @@ __global__ __launch_bounds__(256) void kv4_attn_join(SplitArgs s) {
     s.a.lse[(size_t)row * s.a.n_heads + head] = l != 0.f ? (ref + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
 }
 
-static int attn_tiles(int group, int max_rows) { return (int)std::min<long long>(65535, ((long long)max_rows * group + 15) / 16); }
+// (kv4_prefill_takes leaves at most 1280 + n_kv tiles of all kv heads, or five
+// of each.)
+static int attn_tiles(int group, int max_rows) {
+  return (int)std::min<long long>(65535, ((long long)max_rows * group + 15) / 16);
+}
 // Workgroups that share the axis, of each kv head and column tile.
 template <int D> static int attn_groups(int per_seq) { return std::max(1, ATTN_GROUPS<D> / per_seq); }
 
-size_t kv4_attn_work_bytes(int head_dim, int n_kv, int n_heads, int n_rows, int n_seq, int max_rows, int max_pages) {
+size_t kv4_attn_work_bytes(int head_dim, int n_kv, int n_heads, int n_seq, int max_rows) {
   const int per_seq = n_kv * attn_tiles(n_heads / n_kv, max_rows);
-  const int groups = head_dim == 64 ? attn_groups<64>(per_seq) : head_dim == 128 ? attn_groups<128>(per_seq) : attn_groups<256>(per_seq);
+  const int groups = head_dim == 64 ? attn_groups<64>(per_seq)
+                                    : head_dim == 128 ? attn_groups<128>(per_seq) : attn_groups<256>(per_seq);
   return std::max<size_t>(256, ((size_t)groups + n_seq) * per_seq * (16 * (size_t)head_dim * 4 + 128));
 }
 

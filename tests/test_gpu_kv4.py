@@ -441,6 +441,9 @@ def test_attention_shares_and_parts(case, ty):
     q = _dev(2 * gen.standard_normal((st[-1], heads * dim)).astype(np.float32), ty)
     out, lse = _attend(c, ty, q, st, lens, heads, dim ** -0.5, window)
     _check(c, ty, q, st, lens, heads, dim ** -0.5, window, out, lse)
+    # A bound, no size; the axis is cut by it.
+    out, lse = _attend(c, ty, q, st, lens, heads, dim ** -0.5, window, max_rows=2 ** 31 - 1)
+    _check(c, ty, q, st, lens, heads, dim ** -0.5, window, out, lse)
 
 
 @pytest.mark.parametrize("rows,lens,many", [([1, 1], [200, 40], False), ([40, 3], [100, 40], False),
