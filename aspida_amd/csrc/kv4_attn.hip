@@ -398,11 +398,21 @@ __global__ __launch_bounds__(256) void kv4_attn_join(SplitArgs s) {
   const int max_slots = s.c.max_pages * KV4_PAGE;
   Kv4Span own = {0, 0, 0};
   if (lane < s.rows.n_seq) own = kv4_span(s.rows, lane);
-  const long long share = (axis_total(s.rows, own, s.a.window, max_slots) + s.groups - 1) / s.groups;
-  long long start = lane < b ? rounds_of(own, s.a.window, max_slots) + AXIS_EXTRA : 0;
-  for (int i = 64 + lane; i < b; i += 64) start += rounds_of(kv4_span(s.rows, i), s.a.window, max_slots) + AXIS_EXTRA;
+  long long total, start;  // the axis, and where this sequence begins on it
+  if (s.rows.n_seq <= 64) {
+    const int n = lane < s.rows.n_seq ? rounds_of(own, s.a.window, max_slots) + AXIS_EXTRA : 0;
+    const int upto = wave_scan_add(n);
+    total = __builtin_amdgcn_readlane(upto, 63);
+    start = __builtin_amdgcn_readlane(upto, b) - __builtin_amdgcn_readlane(n, b);
+  } else {
+    total = axis_total(s.rows, own, s.a.window, max_slots);
+    start = lane < b ? rounds_of(own, s.a.window, max_slots) + AXIS_EXTRA : 0;
+    for (int i = 64 + lane; i < b; i += 64)
+      start += rounds_of(kv4_span(s.rows, i), s.a.window, max_slots) + AXIS_EXTRA;
 #pragma unroll
-  for (int o = 32; o; o >>= 1) start += __shfl_xor(start, o, 64);
+    for (int o = 32; o; o >>= 1) start += __shfl_xor(start, o, 64);
+  }
+  const long long share = (total + s.groups - 1) / s.groups;
   start += AXIS_EXTRA;
   const long long first = start / share, last = (start + rounds_of(sp, s.a.window, max_slots) - 1) / share;
   const int count = (int)(last - first) + 1;
