@@ -566,7 +566,10 @@ __global__ __launch_bounds__(1024) void kv4_select(Kv4Evict e, int n_kv) {
   }
 }
 
-// One workgroup per (page of 64 new slots, kv head, sequence).  The key codes
+// One workgroup per (page of 64 new slots, kv head, sequence).  Bound by the
+// lines that it touches: slots kept here and there leave few lines of the old
+// pages unread, whose pieces are 16 bytes a token (35 us of an eviction that
+// writes 42 MB).  The key codes
 // of a token are 16 bytes per lane group and quad and its key scales lie
 // together; a value dword, and the 16 bytes of its scales, collect one entry
 // from each of eight old tokens.  Slots of a page that the source's table does

@@ -68,7 +68,7 @@ struct PageIds {
 };
 
 // A load that leaves nothing in the caches: a cache is read once a step (64
-// lanes of up to 8192 slots 85 -> 80 us; heads of 256 that the caches could
+// lanes of up to 8000 slots 85 -> 80 us; heads of 256 that the caches could
 // have held, 8 lanes of 8000, 35 -> 37).
 template <class V> __device__ __forceinline__ V kv_stream(const uint8_t* p) {
   return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));

@@ -1,9 +1,9 @@
 // kv4_prefill.hip -- attention of many rows over the 4-bit cache.
 //
 // A workgroup takes 32 columns (rows times query heads of one kv head) per
-// wave and walks the pages that they see.  The waves turn a page's codes into
-// f16 operands in LDS once (exact, kv4_mma.h), in the order the 32x32x16
-// instructions read them, while the page before is multiplied; per 32 tokens
+// wave and walks the slots that they see in stages of 32 tokens.  The waves
+// turn a stage's codes into f16 operands in LDS once (exact, kv4_mma.h), in
+// the order the 32x32x16 instructions read them, two stages ahead; per stage
 //   S[token][col] = K Q^T      D / 16 steps, and one for the minima
 //   P = exp2(S - ref)          ref moves when a score passes it by 2^15
 //   O[dim][col] += V^T P       P in S's own registers: the steps' token order
@@ -13,8 +13,13 @@
 // less 8 (d (q - 8), with m + 8 d as two f16 in place of m): the sums over
 // thousands of slots then stay near the result instead of cancelling against
 // the minima (6000 slots: error 3.1e-6 before, of 1.5e-6 in plain f32).
-// Bound by the matrix cores and exp2: a 32 x 32 tile of S is 19 steps of 32
-// cycles (D = 128, one plane) against about 400 cycles of vector work.
+// Bound by issue: the matrix cores are busy 37% of the time, the vector units
+// 43% (unpacking, exp2, the planes of P, address sums), LDS 26%, two waves a
+// SIMD in turns.  2000 rows behind 4000 slots (32/8 heads of 128, f32, 328
+// GFLOP of two planes) 383 us, 860 TFLOP/s; prompts up to 4097 rows (bf16,
+// 391 GFLOP) 557 us, 700 TFLOP/s; a large f16 product reaches 1108.  Measured
+// and not taken: four waves a workgroup, priorities of waves, dwords instead
+// of 16-byte pieces per unpacking thread (598 us for 557).
 #include <algorithm>
 
 #include "kv4_mma.h"

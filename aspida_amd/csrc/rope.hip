@@ -4,7 +4,9 @@
 // by all heads of a token.  A workgroup takes some tokens and some of their
 // heads: it forms the tokens' sin and cos once (f64 angles, f32 results) in
 // LDS, then each thread rotates 16 bytes of one half and 16 of the other
-// (half layout) or 16 bytes of neighbours (interleaved) at a time.
+// (half layout) or 16 bytes of neighbours (interleaved) at a time.  4001 tokens
+// of 72 heads of 128 (bf16, 64 values of each rotated, 147 MB) take 31 us,
+// 4.7 TB/s, of 29 at the rate of a large copy.
 #include "rope.h"
 
 #include <algorithm>
