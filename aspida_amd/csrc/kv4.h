@@ -36,7 +36,9 @@ constexpr int KV4_PAGE = 64;
 constexpr float KV4_D_MAX = 254.f;
 
 __host__ __device__ constexpr int kv4_head_bytes(int head_dim) { return 80 * head_dim; }
-__host__ __device__ constexpr int kv4_bit(int j) { return (((j & 1) << 4) + ((j >> 1) == 0 ? 6 : (j >> 1) == 1 ? 2 : (j >> 1) == 2 ? 14 : 10)) & 31; }
+__host__ __device__ constexpr int kv4_bit(int j) {
+  return (((j & 1) << 4) + ((j >> 1) == 0 ? 6 : (j >> 1) == 1 ? 2 : (j >> 1) == 2 ? 14 : 10)) & 31;
+}
 
 // A cache as the kernels see it.
 struct Kv4View {

@@ -467,7 +467,8 @@ static hipError_t prefill_go(const PrefillArgs& s, hipStream_t st) {
                                            hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) return e;
   const long long tiles = ((long long)std::min(s.a.max_rows, s.rows.n_rows) * s.group + 32 * WAVES - 1) / (32 * WAVES);
-  hipLaunchKernelGGL((kv4_prefill<D, T, WAVES>), dim3(s.c.n_kv, (unsigned)tiles, s.rows.n_seq), dim3(64 * WAVES), lds, st, s);
+  const dim3 grid(s.c.n_kv, (unsigned)tiles, s.rows.n_seq);
+  hipLaunchKernelGGL((kv4_prefill<D, T, WAVES>), grid, dim3(64 * WAVES), lds, st, s);
   return hipGetLastError();
 }
 

@@ -117,7 +117,8 @@ __global__ __launch_bounds__(64 * ONE_WAVES) void kv4_weigh_one(WeighArgs s) {
   };
   load(t0);
   Query<D, TWO> q;
-  q.load((const T*)s.w.q + (size_t)(sp.r0 + (valid ? row : 0)) * s.w.q_stride + (size_t)head * D, valid && any_hi > 0, lane);
+  q.load((const T*)s.w.q + (size_t)(sp.r0 + (valid ? row : 0)) * s.w.q_stride + (size_t)head * D,
+         valid && any_hi > 0, lane);
   const float unit = n > s.w.max_rows ? __builtin_nanf("") : q.unit * (s.w.scale * WEIGH_LOG2E);
   // A row that saw nothing (lse -inf) gives nothing, nor does a column that is none.
   const float lse = valid ? s.w.lse[(size_t)(sp.r0 + row) * s.w.n_heads + head] : -INFINITY;
@@ -200,7 +201,8 @@ __global__ __launch_bounds__(64 * WEIGH_WAVES) void kv4_weigh_many(WeighArgs s) 
       // A row that saw nothing (lse -inf) gives nothing, nor does a column that is none.
       const float lse = valid ? s.w.lse[(size_t)(sp.r0 + row) * s.w.n_heads + head] : -INFINITY;
       const int chi = valid ? max(pos + 1, 0) : 0, clo = s.w.window > 0 ? max(0, pos - s.w.window + 1) : 0;
-      cols[i * 16 + col] = kvu4{__builtin_bit_cast(uint32_t, n > s.w.max_rows ? __builtin_nanf("") : q.unit * (s.w.scale * WEIGH_LOG2E)),
+      const float unit = n > s.w.max_rows ? __builtin_nanf("") : q.unit * (s.w.scale * WEIGH_LOG2E);
+      cols[i * 16 + col] = kvu4{__builtin_bit_cast(uint32_t, unit),
                                 __builtin_bit_cast(uint32_t, lse == -INFINITY ? INFINITY : lse * WEIGH_LOG2E),
                                 (uint32_t)clo, (uint32_t)chi};
     }
@@ -295,7 +297,8 @@ static hipError_t weigh_go(const WeighArgs& s, hipStream_t st) {
   const long long pages = (s.w.acc_stride + KV4_PAGE - 1) / KV4_PAGE;
   const long long most = (pages + WEIGH_WAVES - 1) / WEIGH_WAVES;
   const long long want = (1024 + (long long)s.c.n_kv * s.rows.n_seq - 1) / ((long long)s.c.n_kv * s.rows.n_seq);
-  const hipError_t e = hipFuncSetAttribute((const void*)&kv4_weigh_many<D, T>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)W::LDS);
+  const hipError_t e = hipFuncSetAttribute((const void*)&kv4_weigh_many<D, T>,
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)W::LDS);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((kv4_weigh_many<D, T>), dim3((unsigned)std::min(most, want), s.c.n_kv, s.rows.n_seq),
                      dim3(64 * WEIGH_WAVES), W::LDS, st, s);

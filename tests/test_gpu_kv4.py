@@ -288,6 +288,33 @@ def test_append_of_ties_constants_and_values_beyond_the_format():
             assert np.array_equal(g, want.astype(np.float32).astype(np.float64), equal_nan=True)
 
 
+def test_append_ties_that_lost_bits_break():
+    """Values whose difference from the minimum is a tie after its rounding to
+    f32 but not before: the lost bits decide, not evenness."""
+    gen = np.random.default_rng(2)
+    dim = 64
+    tiny = np.float32(2.0 ** -24)
+    rows = []
+    # Minimum 2^-24, d = 1: n + 1/2 less 2^-24 goes down.  Minimum -2^-24,
+    # d = 1 + 2^-6 (the 7-bit step above 1): (n + 1/2) d and 2^-24 goes up.
+    # Both differences round to the tie from 2 on (ulp 2^-22).
+    for m, d in ((tiny, 1.0), (-tiny, 1.015625)):
+        g = np.full(32, m, np.float32)
+        g[1] = 15.0
+        for n in range(2, 14):
+            g[n] = (n + 0.5) * d
+        rows.append(np.concatenate([g, gen.permutation(g)]))
+    x = np.stack(rows)[:, None]
+    d, _, q = plain.quantise(x)
+    assert (d[0] == 1.0).all() and (d[1] == 1.015625).all()
+    assert (q[0, 0, 0, 2:14] == np.arange(2, 14)).all() and (q[1, 0, 0, 2:14] == np.arange(3, 15)).all()
+    c = Cache(gen, dim, 1, 1, 1)
+    c.append(aa.F32, _dev(x), _dev(x), [0, 2], [2])
+    k, v = c.all([2])[0]
+    want = plain.stands_for(x).astype(np.float32)  # d q + m rounded once, as it is read (3 + 2^-24 is no f32)
+    assert (k == want).all() and (v == want).all()
+
+
 def test_append_leaves_the_rest_alone():
     """Slots before and behind the new rows, other pages, and slots that the
     table does not have (page -1, a page past the pool, more slots than pages)."""
