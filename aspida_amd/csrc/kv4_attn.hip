@@ -25,7 +25,7 @@
 // instructions (unpacking, exp2, the two planes of P) in 1800 cycles, with
 // two waves a SIMD, and 45 matrix instructions beside them.  130001 slots of 8
 // kv heads of 128 (f32, 166 MB) take 42 us, 4.0 TB/s, of 32 at the rate of a
-// large copy; 64 lanes of up to 8000 slots (bf16, 330 MB) 74 us, 4.5 TB/s.
+// large copy; 64 lanes of up to 8000 slots (bf16, 330 MB) 77 us, 4.3 TB/s.
 #include <algorithm>
 
 #include "kv4_mma.h"
