@@ -14,7 +14,9 @@
 //   O[dim][col] += V^T P    P in S's own registers: S's lane holds tokens 4 rg
 //                           + 0..3 of two tiles for one column, which is how
 //                           the value dwords are ordered; one more step for
-//                           the minima
+//                           the minima; P is two f16 numbers for every type
+//                           (one leaves 2^-11 of a weight, as much as an f16
+//                           result's own rounding)
 // so nothing passes through LDS until the waves of a workgroup are joined.
 // The sequences' slots stand one after the other on one axis, which is cut
 // into equal shares, one for each workgroup that fits on the card at once: a
@@ -25,7 +27,7 @@
 // instructions (unpacking, exp2, the two planes of P) in 1800 cycles, with
 // two waves a SIMD, and 45 matrix instructions beside them.  130001 slots of 8
 // kv heads of 128 (f32, 166 MB) take 42 us, 4.0 TB/s, of 32 at the rate of a
-// large copy; 64 lanes of up to 8000 slots (bf16, 330 MB) 77 us, 4.3 TB/s.
+// large copy; 64 lanes of up to 8000 slots (bf16, 330 MB) 79 us, 4.2 TB/s.
 #include <algorithm>
 
 #include "kv4_mma.h"
@@ -287,10 +289,10 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, D == 64 ? 3 : D == 128 ? 2 : 1) vo
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], u, -ref));
         l += p;
         ph[j] = (_Float16)p;
-        if constexpr (TWO) pl[j] = (_Float16)(p - (float)ph[j]);
+        pl[j] = (_Float16)(p - (float)ph[j]);
       }
       const kvh8 vm = __builtin_bit_cast(kvh8, y.v.m);
-      if constexpr (TWO) om = kv_mfma(vm, pl, om);
+      om = kv_mfma(vm, pl, om);
       om = kv_mfma(vm, ph, om);
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
@@ -301,7 +303,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, D == 64 ? 3 : D == 128 ? 2 : 1) vo
         for (int e = 0; e < 2; ++e) {
           const int i = 2 * g + e;
           const kvh8 a = kv4_unpack(y.v.w[i >> 2][i & 3], d0, d1, d2, d3, n0, n1, n2, n3);
-          if constexpr (TWO) o[i] = kv_mfma(a, pl, o[i]);
+          o[i] = kv_mfma(a, pl, o[i]);
           o[i] = kv_mfma(a, ph, o[i]);
         }
       }

@@ -9,17 +9,20 @@
 //   O[dim][col] += V^T P       P in S's own registers: the steps' token order
 //                              is the one in which S's lanes hold them
 //   M[g][col] += m^T P         the minima, with a row of ones that sums P
-// f32 activations: two f16 planes of Q and of P, each in turn, and value codes
-// less 8 (d (q - 8), with m + 8 d as two f16 in place of m): the sums over
-// thousands of slots then stay near the result instead of cancelling against
-// the minima (6000 slots: error 3.1e-6 before, of 1.5e-6 in plain f32).
+// P is two f16 planes, each in turn, for every type (one leaves 2^-11 of a
+// weight, as much as an f16 result's own rounding).  f32 activations: two of Q
+// as well, and value codes less 8 (d (q - 8), with m + 8 d as two f16 in place
+// of m): the sums over thousands of slots then stay near the result instead of
+// cancelling against the minima (6000 slots: error 3.1e-6 before, of 1.5e-6 in
+// plain f32).
 // Bound by issue: the matrix cores are busy 37% of the time, the vector units
 // 43% (unpacking, exp2, the planes of P, address sums), LDS 26%, two waves a
 // SIMD in turns.  2000 rows behind 4000 slots (32/8 heads of 128, f32, 328
 // GFLOP of two planes) 383 us, 860 TFLOP/s; prompts up to 4097 rows (bf16,
-// 391 GFLOP) 557 us, 700 TFLOP/s; a large f16 product reaches 1108.  Measured
-// and not taken: four waves a workgroup, priorities of waves, dwords instead
-// of 16-byte pieces per unpacking thread (598 us for 557).
+// 391 GFLOP and half as many for P's low plane) 672 us, 870 TFLOP/s; a large
+// f16 product reaches 1108.  Measured and not taken: four waves a workgroup,
+// priorities of waves, dwords instead of 16-byte pieces per unpacking thread
+// (with one plane of P 598 us for 557).
 #include <algorithm>
 
 #include "kv4_mma.h"
@@ -287,9 +290,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(Pr
   for (int i = 0; i < NG; ++i) o[i] = om;
   // A row past the table sees its own slot there: NaN.
   float ref = -3.402823466e38f;
-  // The ones row sums P as the products see it, which is what o is divided by;
-  // with one plane those are rounded weights, and lse takes the unrounded sum.
-  float lsum = 0.f;
   const bool past = chi > max_slots;
 
   // Rows of the value minima that no group has: zeros, and ones in row 8.
@@ -359,7 +359,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(Pr
 #pragma unroll
       for (int i = 0; i < NG; ++i) o[i] *= f;
       om *= f;
-      lsum *= f;
     }
   };
   // One stage: its weights from the scores c, the next one's scores into c2.
@@ -374,9 +373,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(Pr
       for (int j = 0; j < 8; ++j) {
         x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(c[8 * e + j], u, -ref));
         ph[e][j] = (_Float16)x[j];
-        if constexpr (TWO) pl[e][j] = (_Float16)(x[j] - (float)ph[e][j]);
+        pl[e][j] = (_Float16)(x[j] - (float)ph[e][j]);
       }
-      if constexpr (!TWO) lsum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -384,13 +382,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(Pr
       if constexpr (TWO) {
         const kvh8 vl = *reinterpret_cast<const kvh8*>(pg + P::VL + e * 512 + (hl * 16 + (col & 15)) * 16);
         om = kv_mfma32(vl, ph[e], om);
-        om = kv_mfma32(vm, pl[e], om);
       }
+      om = kv_mfma32(vm, pl[e], om);
       om = kv_mfma32(vm, ph[e], om);
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         const kvh8 v = *reinterpret_cast<const kvh8*>(pg + P::V + g * 2048 + e * 1024 + lane * 16);
-        if constexpr (TWO) o[g] = kv_mfma32(v, pl[e], o[g]);
+        o[g] = kv_mfma32(v, pl[e], o[g]);
         o[g] = kv_mfma32(v, ph[e], o[g]);
       }
     }
@@ -444,7 +442,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(Pr
       __builtin_memcpy(out + 32 * g + 8 * i, &r, sizeof(r));
     }
   }
-  if (!TWO) l = lsum + __shfl_xor(lsum, 32, 64) + (past ? l : 0.f);
   if (valid && s.a.lse && hl == 0)
     s.a.lse[(size_t)(sp.r0 + row) * s.a.n_heads + head] = l != 0.f ? (ref + __builtin_amdgcn_logf(l)) * PF_LN2 : -INFINITY;
   // Rows past max_rows have no workgroup: NaN, by the first tile's.
