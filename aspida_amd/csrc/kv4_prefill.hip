@@ -18,7 +18,7 @@
 // Bound by issue: the matrix cores are busy 37% of the time, the vector units
 // 43% (unpacking, exp2, the planes of P, address sums), LDS 26%, two waves a
 // SIMD in turns.  2000 rows behind 4000 slots (32/8 heads of 128, f32, 328
-// GFLOP of two planes) 383 us, 860 TFLOP/s; prompts up to 4097 rows (bf16,
+// GFLOP of two planes) 385 us, 850 TFLOP/s; prompts up to 4097 rows (bf16,
 // 391 GFLOP and half as many for P's low plane) 672 us, 870 TFLOP/s; a large
 // f16 product reaches 1108.  Measured and not taken: four waves a workgroup,
 // priorities of waves, dwords instead of 16-byte pieces per unpacking thread
@@ -175,7 +175,9 @@ template <int D, bool TWO> struct StageLoad {
         for (int j = 0; j < 4; ++j) {
           const kvh2 mj = kv_h2(mm[j]), dj = kv_h2(md[j]);
           const float a = __builtin_fmaf(8.f, (float)dj.x, (float)mj.x), b = __builtin_fmaf(8.f, (float)dj.y, (float)mj.y);
-          const kvh2 hi2 = {(_Float16)a, (_Float16)b}, lo2 = {(_Float16)(a - (float)hi2.x), (_Float16)(b - (float)hi2.y)};
+          // m + 8 d may pass f16's largest value by 2032, which the low number then holds.
+          const kvh2 hi2 = {(_Float16)fminf(a, 65504.f), (_Float16)fminf(b, 65504.f)};
+          const kvh2 lo2 = {(_Float16)(a - (float)hi2.x), (_Float16)(b - (float)hi2.y)};
           mm[j] = __builtin_bit_cast(uint32_t, hi2);
           low[j] = __builtin_bit_cast(uint32_t, lo2);
         }
@@ -381,6 +383,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(Pr
       const kvh8 vm = *reinterpret_cast<const kvh8*>(pg + P::VM + e * 512 + (hl * 16 + (col & 15)) * 16);
       if constexpr (TWO) {
         const kvh8 vl = *reinterpret_cast<const kvh8*>(pg + P::VL + e * 512 + (hl * 16 + (col & 15)) * 16);
+        om = kv_mfma32(vl, pl[e], om);
         om = kv_mfma32(vl, ph[e], om);
       }
       om = kv_mfma32(vm, pl[e], om);

@@ -7,7 +7,7 @@ import pytest
 import aspida_amd as aa
 import kv4_accuracy as acc
 import kv4_plain as plain
-from test_gpu_kv4 import NAMES, _attend, _dev, _filled, _host, _starts
+from test_gpu_kv4 import NAMES, Cache, _attend, _check, _dev, _filled, _host, _kv, _starts
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +46,30 @@ def test_attention_is_as_accurate_as_f32(case, ty):
         assert acc.over(ho, wo, o32) <= 1
     else:
         assert acc.over16(ho, wo, o32, BITS[ty]) <= 1
+
+
+@pytest.mark.parametrize("rows,many", [(3, False), (90, True)], ids=["few", "many"])
+@pytest.mark.parametrize("ty", [aa.F32, aa.BF16], ids=NAMES.get)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attention_of_values_at_the_ends_of_f16(dim, ty, rows, many):
+    """Groups whose minimum, and whose minimum and half its range, lie at f16's
+    largest values or beyond them, in sight of some of the rows."""
+    gen = np.random.default_rng(dim)
+    heads, kv, n = 8, 2, 150
+    k, v = _kv(gen, n, kv, dim)
+    g = v.reshape(n, kv, dim // 32, 32)
+    codes = np.concatenate([np.arange(16), np.arange(16)]).astype(np.float32)
+    g[n - 20, :, 1] = 64000 + 250 * gen.permutation(codes)
+    g[n - 50, 0, 0] = -65504 + 254 * gen.permutation(codes)
+    g[n - 1, 1, 0] = 65504 + 254 * gen.permutation(codes)
+    c = Cache(gen, dim, kv, 1, 3)
+    c.append(aa.F32, _dev(k), _dev(v), [0, n], [n])
+    kvs = c.all([n])
+    assert np.isfinite(kvs[0][1]).all() and kvs[0][1].max() == 65504 + 15 * 254
+    q, scale = _dev(2 * gen.standard_normal((rows, heads * dim)).astype(np.float32), ty), dim ** -0.5
+    out, lse = _attend(c, ty, q, [0, rows], [n], heads, scale, many=many)
+    _check(c, ty, q, [0, rows], [n], heads, scale, 0, out, lse, kvs)
+    if ty == aa.F32:
+        hq = _host(q).reshape(rows, heads, dim)
+        want = plain.attend(hq, *kvs[0], scale)[0]
+        assert acc.over(_host(out).reshape(want.shape), want, acc.attend32(hq, *kvs[0], scale)[0]) <= 1
