@@ -443,11 +443,10 @@ __device__ __forceinline__ int wg_before(int v, int* part, int* total) {
 // One workgroup per (kv head, sequence): the rank of the lightest slot kept,
 // by the 31 bits of a weight from the top (a histogram of the slots still in
 // question per 11, 10 and 10 of them), then the kept slots in order.  Among
-// slots of that rank the lowest stay.  new_len is the same for every head;
-// head 0 writes it.  Bound by latencies, the weights being in cache after the
-// first pass: eight are in flight per thread, bins are summed by all threads
-// (by one thread, 256 bins: 56 us at 16 x 8 rows of 8193, now 12), and the
-// ranks of 8192 slots come from ballots and one barrier.
+// slots of that rank the lowest stay.  Bound by latencies, the weights being in
+// cache after the first pass: eight are in flight per thread, bins are summed
+// by all threads (by one thread, 256 bins: 56 us at 16 x 8 rows of 8193, now
+// 12), and the ranks of 8192 slots come from ballots and one barrier.
 __global__ __launch_bounds__(1024) void kv4_select(Kv4Evict e, int n_kv) {
   constexpr int PER = 8;
   __shared__ int hist[2048];
@@ -470,7 +469,6 @@ __global__ __launch_bounds__(1024) void kv4_select(Kv4Evict e, int n_kv) {
     for (int j = 0; j < PER; ++j)
       if (i0 + 64 * (PER * wave + j) + lane >= have) v[j] = 0.f;
   };
-  if (hk == 0 && tid == 0) e.new_len[b] = kept;
   for (int i = kept + tid; i < e.keep; i += 1024) {
     idx[i] = -1;
     out[i] = 0.f;
@@ -574,7 +572,9 @@ __global__ __launch_bounds__(1024) void kv4_select(Kv4Evict e, int n_kv) {
 // together; a value dword, and the 16 bytes of its scales, collect one entry
 // from each of eight old tokens.  Slots of a page that the source's table does
 // not have read as NaN: key steps of NaN, all else 0.  What stands in new
-// slots past the last one is 0 where a word shares it.
+// slots past the last one is 0 where a word shares it.  The first page's
+// workgroup of head 0 writes new_len: it may be kv_len, for here, unlike in
+// the selection, both its values give the same slots.
 template <int D>
 __global__ __launch_bounds__(256) void kv4_gather(Kv4View src, Kv4View dst, Kv4Evict e) {
   using L = Kv4L<D>;
@@ -584,6 +584,7 @@ __global__ __launch_bounds__(256) void kv4_gather(Kv4View src, Kv4View dst, Kv4E
   const int hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   const int kept = min(max(e.kv_len[b], 0), e.keep);
   const int s0 = blockIdx.x * KV4_PAGE;
+  if (s0 == 0 && hk == 0 && tid == 0) e.new_len[b] = kept;
   if (s0 >= kept) return;
   uint8_t* to = kv4_block(dst, b, blockIdx.x, hk, L::BYTES);
   if (!to) return;

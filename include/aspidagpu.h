@@ -343,7 +343,8 @@ int aspida_kv4_weigh_dev(const aspida_kv4 *cache, int type, const void *q, long 
  * heaviest by acc (NaN, negative and missing weights count as 0), among equals
  * the lowest; they move in order to slots 0 .. keep - 1 of dst's pages (same
  * head_dim and n_kv, its own table, no page in common with what src's table
- * names).  Shorter sequences are copied.  new_len[n_seq] = min(kv_len, keep);
+ * names).  Shorter sequences are copied.  new_len[n_seq] = min(kv_len, keep)
+ * (it may be kv_len, for lengths that shrink in place);
  * idx and acc_out [n_seq][n_kv][keep] hold the old slot and weight of each
  * new one, -1 and 0 past new_len.  first + recent <= keep. */
 int aspida_kv4_evict_dev(const aspida_kv4 *src, int n_seq, const int *kv_len, const float *acc, long long acc_stride,
