@@ -2,8 +2,9 @@
 import numpy as np
 import pytest
 
+import aspida_amd as aa
 from gpu_helpers import stream, sync, torch_cuda
-from test_gpu_kv4 import Cache, _dev, _filled, _i32
+from test_gpu_kv4 import Cache, _attend, _dev, _filled, _host, _i32
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +30,26 @@ def test_evict_shrinks_lengths_in_place():
         results.append((idx, out, dst.pages))
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("window", [0, 3])
+@pytest.mark.parametrize("rows,heads", [(10, 4), (40, 1), (20, 8)])
+def test_slot_weights_past_max_rows_are_nan_in_every_slot_seen(rows, heads, window):
+    """Also in slots that only rows past the first 16 columns see, and in no others."""
+    torch = torch_cuda()
+    gen = np.random.default_rng(3)
+    lens = [100, 80]
+    c = _filled(gen, 128, 1, lens)
+    q = _dev(gen.standard_normal((rows + 1, heads * 128)).astype(np.float32))
+    st = [0, rows, rows + 1]
+    _, lse = _attend(c, aa.F32, q, st, lens, heads, 0.1, window)
+    base = gen.random((2, 1, 128)).astype(np.float32)
+    a, out = _dev(base), torch.zeros(2, 1, 128, device="cuda")
+    s, l = _i32(st), _i32(lens)
+    for max_rows in (1, rows - 1):
+        c.dev.kv4_weigh(c.c, aa.F32, q.data_ptr(), heads * 128, heads, rows + 1, 2, s.data_ptr(), max_rows, l.data_ptr(),
+                        0.1, lse.data_ptr(), a.data_ptr(), out.data_ptr(), 128, stream(), window=window)
+        sync()
+        o, lo = _host(out)[:, 0], max(0, 100 - rows - window + 1) if window else 0
+        assert np.isnan(o[0, lo:100]).all() and np.isfinite(o[1]).all()
+        assert np.array_equal(o[0, :lo], base[0, 0, :lo]) and np.array_equal(o[0, 100:], base[0, 0, 100:])
