@@ -166,6 +166,12 @@ __device__ __forceinline__ Kv4Span kv4_span(const Kv4Rows& r, int b) {
   return s;
 }
 
+// The lowest slot that the row at slot `pos` sees, where `reach` slots before
+// its own are in the window (kv4_reach).  Rows below 0 see none; windows may
+// be up to INT_MAX.
+__device__ __forceinline__ int kv4_reach(int window) { return window > 0 ? window - 1 : 0x7FFFFFFF; }
+__device__ __forceinline__ int kv4_lowest(int pos, int reach) { return max(0, max(pos, 0) - reach); }
+
 __device__ __forceinline__ uint32_t kv4_code(uint32_t w, int j) {
   return __builtin_amdgcn_alignbit(w, w, (uint32_t)kv4_bit(j)) & 15u;
 }

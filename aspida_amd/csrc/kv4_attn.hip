@@ -54,7 +54,7 @@ __device__ __forceinline__ SeenRange seen_range(const Kv4Span& s, int window, in
   const int first = s.len - (s.r1 - s.r0);  // the first row's slot
   SeenRange r;
   r.hi = s.r1 > s.r0 ? min(s.len, max_slots) : 0;
-  r.lo = window > 0 ? min(max(0, first - window + 1) & ~31, r.hi & ~31) : 0;
+  r.lo = min(kv4_lowest(first, kv4_reach(window)), r.hi) & ~31;
   return r;
 }
 
@@ -210,17 +210,18 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, D == 64 ? 3 : D == 128 ? 2 : 1) vo
     const int ncol = min(16, min(n, s.a.max_rows) * s.group - tile * 16);
     if (ncol <= 0) continue;
     // This lane's column: its row, head, and the slots [clo, chi) it sees.
+    const int reach = kv4_reach(s.a.window);
     const int ci = tile * 16 + col, row = ci / s.group, head = hk * s.group + ci % s.group;
     const bool valid = col < ncol;
     const int pos = sp.len - n + row;
-    const int chi = valid ? max(pos + 1, 0) : 0, clo = s.a.window > 0 ? max(0, pos - s.a.window + 1) : 0;
+    const int chi = valid ? max(pos + 1, 0) : 0, clo = kv4_lowest(pos, reach);
     // The share's slots, and those of them that every column sees.
     const int t0 = seen.lo + u0 * ATTN_STEP, t1 = (int)min((long long)seen.hi, seen.lo + (long long)u1 * ATTN_STEP);
     const int row_last = (tile * 16 + ncol - 1) / s.group, row_first = tile * 16 / s.group;
     const int all_hi = sp.len - n + row_first + 1;                                       // below: seen by every column
-    const int all_lo = s.a.window > 0 ? max(0, sp.len - n + row_last - s.a.window + 1) : 0;
+    const int all_lo = kv4_lowest(sp.len - n + row_last, reach);
     const int any_hi = min(t1, sp.len - n + row_last + 1);
-    const int any_lo = s.a.window > 0 ? max(0, sp.len - n + row_first - s.a.window + 1) : 0;
+    const int any_lo = kv4_lowest(sp.len - n + row_first, reach);
 
     kvf4 o[NT], om = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll

@@ -215,18 +215,18 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(Pr
   if (tile < 0) return;
   const int c0 = tile * COLS, c1 = min(c0 + COLS, nr * s.group);  // the workgroup's columns
   const int first = sp.len - n;                                   // slot of row 0
-  const int max_slots = s.c.max_pages * KV4_PAGE;
+  const int max_slots = s.c.max_pages * KV4_PAGE, reach = kv4_reach(s.a.window);
   const int any_hi = min(first + (c1 - 1) / s.group + 1, max_slots);
-  const int any_lo = s.a.window > 0 ? max(0, first + c0 / s.group - s.a.window + 1) : 0;
+  const int any_lo = kv4_lowest(first + c0 / s.group, reach);
 
   // This lane's column, and what the wave's columns all see and see at all.
   const int w0 = c0 + 32 * wave, w1 = min(w0 + 32, c1) - 1;
   const int ci = w0 + col, row = ci / s.group, head = hk * s.group + ci % s.group;
   const bool valid = ci < c1;
   const int pos = first + row;
-  const int chi = valid ? max(pos + 1, 0) : 0, clo = s.a.window > 0 ? max(0, pos - s.a.window + 1) : 0;
+  const int chi = valid ? max(pos + 1, 0) : 0, clo = kv4_lowest(pos, reach);
   const int all_hi = first + w0 / s.group + 1;
-  const int all_lo = s.a.window > 0 ? max(0, first + max(w1, w0) / s.group - s.a.window + 1) : 0;
+  const int all_lo = kv4_lowest(first + max(w1, w0) / s.group, reach);
 
   // f32 activations with a head of 128: the low plane of Q would not fit in
   // the registers of two waves per SIMD and is read from LDS.

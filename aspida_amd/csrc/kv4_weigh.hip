@@ -87,16 +87,16 @@ __global__ __launch_bounds__(64 * ONE_WAVES) void kv4_weigh_one(WeighArgs s) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hk = blockIdx.y, b = blockIdx.z;
   const Kv4Span sp = kv4_span(s.rows, b);
-  const int n = sp.r1 - sp.r0, first = sp.len - n;
-  const int any_lo = s.w.window > 0 ? max(0, first - s.w.window + 1) : 0, any_hi = n > 0 ? sp.len : 0;
+  const int n = sp.r1 - sp.r0, first = sp.len - n, reach = kv4_reach(s.w.window);
+  const int any_lo = kv4_lowest(first, reach), any_hi = n > 0 ? sp.len : 0;
   const size_t at = ((size_t)b * s.c.n_kv + hk) * s.w.acc_stride;
   const float* in = s.w.acc_in ? s.w.acc_in + at : nullptr;
   float* out = s.w.acc_out + at;
   const int row = col / s.group, head = hk * s.group + col % s.group;
   const bool valid = row < n;
-  const int chi = valid ? max(first + row + 1, 0) : 0, clo = s.w.window > 0 ? max(0, first + row - s.w.window + 1) : 0;
+  const int chi = valid ? max(first + row + 1, 0) : 0, clo = kv4_lowest(first + row, reach);
   // What every column that counts sees (columns that are none have lse inf).
-  const int all_hi = first + 1, all_lo = s.w.window > 0 ? max(0, first + min(n - 1, 15 / s.group) - s.w.window + 1) : 0;
+  const int all_hi = first + 1, all_lo = kv4_lowest(first + min(n - 1, 15 / s.group), reach);
 
   const long long step = (long long)gridDim.x * ONE_WAVES * TOK;
   long long t0 = ((long long)blockIdx.x * ONE_WAVES + wave) * TOK;
@@ -182,9 +182,9 @@ __global__ __launch_bounds__(64 * WEIGH_WAVES) void kv4_weigh_many(WeighArgs s) 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hk = blockIdx.y, b = blockIdx.z;
   const Kv4Span sp = kv4_span(s.rows, b);
-  const int n = sp.r1 - sp.r0, first = sp.len - n;  // the first row's slot
+  const int n = sp.r1 - sp.r0, first = sp.len - n, reach = kv4_reach(s.w.window);  // first: the first row's slot
   const int tiles = (int)(((long long)n * s.group + 15) / 16);
-  const int any_lo = s.w.window > 0 ? max(0, first - s.w.window + 1) : 0, any_hi = n > 0 ? sp.len : 0;
+  const int any_lo = kv4_lowest(first, reach), any_hi = n > 0 ? sp.len : 0;
   const size_t at = ((size_t)b * s.c.n_kv + hk) * s.w.acc_stride;
   const float* in = s.w.acc_in ? s.w.acc_in + at : nullptr;
   float* out = s.w.acc_out + at;
@@ -206,7 +206,7 @@ __global__ __launch_bounds__(64 * WEIGH_WAVES) void kv4_weigh_many(WeighArgs s) 
     if (rg == 0) {
       // A row that saw nothing (lse -inf) gives nothing, nor does a column that is none.
       const float lse = valid ? s.w.lse[(size_t)(sp.r0 + row) * s.w.n_heads + head] : -INFINITY;
-      const int chi = valid ? max(pos + 1, 0) : 0, clo = s.w.window > 0 ? max(0, pos - s.w.window + 1) : 0;
+      const int chi = valid ? max(pos + 1, 0) : 0, clo = kv4_lowest(pos, reach);
       const float unit = n > s.w.max_rows ? __builtin_nanf("") : q.unit * (s.w.scale * WEIGH_LOG2E);
       cols[i * 16 + col] = kvu4{__builtin_bit_cast(uint32_t, unit),
                                 __builtin_bit_cast(uint32_t, lse == -INFINITY ? INFINITY : lse * WEIGH_LOG2E),
@@ -248,9 +248,8 @@ __global__ __launch_bounds__(64 * WEIGH_WAVES) void kv4_weigh_many(WeighArgs s) 
         for (int i = 0; i < min(W::TILES, tiles - c0); ++i) {
           const int r0 = (c0 + i) * 16 / s.group, r1 = min(n - 1, ((c0 + i) * 16 + 15) / s.group);
           // No row of the tile sees the page: all below it, or their windows past it.
-          if (first + r1 < t0 || (s.w.window > 0 && first + r0 - s.w.window + 1 >= t0 + KV4_PAGE)) continue;
-          const bool whole = there && first + r0 + 1 >= t0 + KV4_PAGE &&
-                             (s.w.window <= 0 || first + r1 - s.w.window + 1 <= t0);
+          if (first + r1 < t0 || max(first + r0, 0) - reach >= t0 + KV4_PAGE) continue;
+          const bool whole = there && first + r0 + 1 >= t0 + KV4_PAGE && max(first + r1, 0) - reach <= t0;
           const kvu4* from = lds + i * W::OPS * 64 + lane;
           Query<D, TWO> q;
           q.sums = __builtin_bit_cast(kvh8, from[0]);

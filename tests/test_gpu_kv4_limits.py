@@ -4,7 +4,7 @@ import pytest
 
 import aspida_amd as aa
 from gpu_helpers import stream, sync, torch_cuda
-from test_gpu_kv4 import Cache, _attend, _dev, _filled, _host, _i32
+from test_gpu_kv4 import Cache, _attend, _dev, _filled, _host, _i32, _starts
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +53,27 @@ def test_slot_weights_past_max_rows_are_nan_in_every_slot_seen(rows, heads, wind
         o, lo = _host(out)[:, 0], max(0, 100 - rows - window + 1) if window else 0
         assert np.isnan(o[0, lo:100]).all() and np.isfinite(o[1]).all()
         assert np.array_equal(o[0, :lo], base[0, 0, :lo]) and np.array_equal(o[0, 100:], base[0, 0, 100:])
+
+
+@pytest.mark.parametrize("rows,many", [([5, 4], False), ([100, 90], True)], ids=["few", "many"])
+def test_windows_beyond_every_slot_hide_nothing(rows, many):
+    """Up to INT_MAX, also for a sequence with rows below slot 0."""
+    torch = torch_cuda()
+    gen = np.random.default_rng(13)
+    dim, heads, kv, lens = 128, 4, 2, [rows[0] - 3, 300]
+    c = _filled(gen, dim, kv, lens, max_pages=5)
+    st = _starts(rows)
+    q = _dev(gen.standard_normal((st[-1], heads * dim)).astype(np.float32))
+    want, wl = _attend(c, aa.F32, q, st, lens, heads, 0.1, many=many)
+    assert np.isfinite(_host(want)).all() and (wl[3:] > -100).all()
+    s, l = _i32(st), _i32(lens)
+    weights = []
+    for window in (0, 5 * 64, 1 << 30, 2 ** 31 - 1):
+        out, lse = _attend(c, aa.F32, q, st, lens, heads, 0.1, window, many=many)
+        assert (out == want).all() and (lse == wl).all()
+        a = torch.zeros(2, kv, 320, device="cuda")
+        c.dev.kv4_weigh(c.c, aa.F32, q.data_ptr(), heads * dim, heads, int(st[-1]), 2, s.data_ptr(), max(rows),
+                        l.data_ptr(), 0.1, lse.data_ptr(), 0, a.data_ptr(), 320, stream(), window=window)
+        sync()
+        weights.append(a)
+    assert all((w == weights[0]).all() for w in weights)
