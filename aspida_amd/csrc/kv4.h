@@ -72,7 +72,7 @@ struct Kv4Attn {
   int n_heads, max_rows, window;
   float scale;
 };
-size_t kv4_attn_work_bytes(int head_dim, int n_kv, int n_heads, int n_seq, int max_rows);
+size_t kv4_attn_work_bytes(int head_dim);
 hipError_t launch_kv4_attn(int head_dim, const Kv4View& c, int type, const Kv4Rows& rows, const Kv4Attn& a,
                            hipStream_t s);
 

@@ -182,7 +182,7 @@ extern "C" long long aspida_kv4_attn_work_bytes(const aspida_kv4* cache, int n_h
                                                 int max_rows) {
   if (!valid_cache(cache) || !valid_heads(cache, n_heads) || n_rows < 0 || n_seq < 0 || n_seq > 65535 || max_rows < 1)
     return -EINVAL;
-  return (long long)kq::kv4_attn_work_bytes(cache->head_dim, cache->n_kv, n_heads, n_seq, longest(max_rows, n_rows));
+  return (long long)kq::kv4_attn_work_bytes(cache->head_dim);
 }
 
 extern "C" int aspida_kv4_attn_dev(const aspida_kv4* cache, int type, const void* q, long long q_stride, int n_heads,

@@ -131,8 +131,9 @@ __device__ __forceinline__ AxisPlace axis_place(const Kv4Rows& rows, const Kv4Sp
 }
 
 // Workspace: per part, kv head and column tile the columns' sums [16][D] and
-// (ref, l) [16].  Workgroup x's part of sequence b is number x + b: along the
-// axis one or the other grows.
+// (ref, l) [16].  A workgroup has at most two sequences in part: one that
+// began in a share before its own (number 2 x) and one that goes on in the
+// next (2 x + 1), so parts number as the workgroups do, not as the sequences.
 template <int D> struct AttnPart {
   float o[16][D];
   float ref[16], l[16];
@@ -379,7 +380,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, D == 64 ? 3 : D == 128 ? 2 : 1) vo
         s.a.lse[(size_t)(sp.r0 + row) * s.a.n_heads + head] = l != 0.f ? (ref + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
       continue;
     }
-    AttnPart<D>* part = (AttnPart<D>*)s.a.work + ((size_t)blockIdx.x + b) * gridDim.y + blockIdx.y;
+    AttnPart<D>* part = (AttnPart<D>*)s.a.work + (2 * (size_t)blockIdx.x + (u0 == 0)) * gridDim.y + blockIdx.y;
 #pragma unroll
     for (int i = 0; i < NT; ++i) *reinterpret_cast<kvf4*>(&part->o[col][16 * i + 4 * rg]) = o[i];
     if (rg == 0) { part->ref[col] = ref; part->l[col] = l; }
@@ -420,15 +421,17 @@ __global__ __launch_bounds__(256) void kv4_attn_join(SplitArgs s) {
   const long long first = start / share, last = (start + rounds_of(sp, s.a.window, max_slots) - 1) / share;
   const int count = (int)(last - first) + 1;
   if (count == 1) return;
-  const AttnPart<D>* part = (const AttnPart<D>*)s.a.work + (size_t)(first + b) * gridDim.y + blockIdx.y;
+  // Its parts: number 2 first + 1, then 2 x of the workgroups behind.
   const size_t step = gridDim.y;
+  const AttnPart<D>* parts = (const AttnPart<D>*)s.a.work + 2 * (size_t)first * step + blockIdx.y;
+  auto part = [&](int i) -> const AttnPart<D>& { return parts[(i ? 2 * (size_t)i : 1) * step]; };
   float ref = REF0;
-  for (int i = lane; i < count; i += 64) ref = fmaxf(ref, part[i * step].ref[col]);
+  for (int i = lane; i < count; i += 64) ref = fmaxf(ref, part(i).ref[col]);
   for (int o = 32; o; o >>= 1) ref = fmaxf(ref, __shfl_xor(ref, o, 64));
   float l = 0.f, y[E] = {};
 #pragma unroll 8
   for (int i = wave; i < count; i += 4) {
-    const AttnPart<D>& p = part[i * step];
+    const AttnPart<D>& p = part(i);
     const float f = __builtin_amdgcn_exp2f(p.ref[col] - ref);
     l += p.l[col] * f;
 #pragma unroll
@@ -456,11 +459,13 @@ static int attn_tiles(int group, int max_rows) {
 // Workgroups that share the axis, of each kv head and column tile.
 template <int D> static int attn_groups(int per_seq) { return std::max(1, ATTN_GROUPS<D> / per_seq); }
 
-size_t kv4_attn_work_bytes(int head_dim, int n_kv, int n_heads, int n_seq, int max_rows) {
-  const int per_seq = n_kv * attn_tiles(n_heads / n_kv, max_rows);
-  const int groups = head_dim == 64 ? attn_groups<64>(per_seq)
-                                    : head_dim == 128 ? attn_groups<128>(per_seq) : attn_groups<256>(per_seq);
-  return std::max<size_t>(256, ((size_t)groups + n_seq) * per_seq * (16 * (size_t)head_dim * 4 + 128));
+// Two parts of each workgroup, and workgroups times column tiles are at most
+// ATTN_GROUPS: with more tiles one workgroup walks the whole axis, and there
+// are no parts.
+size_t kv4_attn_work_bytes(int head_dim) {
+  return head_dim == 64    ? 2 * ATTN_GROUPS<64> * sizeof(AttnPart<64>)
+         : head_dim == 128 ? 2 * ATTN_GROUPS<128> * sizeof(AttnPart<128>)
+                           : 2 * ATTN_GROUPS<256> * sizeof(AttnPart<256>);
 }
 
 template <int D, class T>

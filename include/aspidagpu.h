@@ -320,8 +320,9 @@ int aspida_kv4_read_dev(const aspida_kv4 *cache, int type, int n_rows, int n_seq
  * sees nothing (kv_len 0, or a slot below 0) gets 0, and lse -inf; what masked
  * slots hold never matters.  max_rows: at least the rows of the longest
  * sequence (what a sequence has past it comes out as NaN).  work: 256-byte
- * aligned, aspida_kv4_attn_work_bytes for the same arguments; launches that
- * share it must be ordered.  out must not overlap q. */
+ * aligned, aspida_kv4_attn_work_bytes long: 6 to 9 MB, the same for all calls
+ * of a head_dim, so one workspace serves them in turn; launches that share it
+ * must be ordered.  out must not overlap q. */
 long long aspida_kv4_attn_work_bytes(const aspida_kv4 *cache, int n_heads, int n_rows, int n_seq, int max_rows);
 int aspida_kv4_attn_dev(const aspida_kv4 *cache, int type, const void *q, long long q_stride, int n_heads, int n_rows,
                         int n_seq, const int *row_start, int max_rows, const int *kv_len, float scale, int window,

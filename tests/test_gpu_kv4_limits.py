@@ -4,7 +4,7 @@ import pytest
 
 import aspida_amd as aa
 from gpu_helpers import stream, sync, torch_cuda
-from test_gpu_kv4 import Cache, _attend, _dev, _filled, _host, _i32, _starts
+from test_gpu_kv4 import Cache, _attend, _check, _dev, _filled, _host, _i32, _starts
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +77,31 @@ def test_windows_beyond_every_slot_hide_nothing(rows, many):
         sync()
         weights.append(a)
     assert all((w == weights[0]).all() for w in weights)
+
+
+@pytest.mark.parametrize("dim,heads,kv,rows,lens", [
+    (64, 4, 1, [1], [9001]), (64, 64, 8, [1] * 70, [(131 * i) % 900 for i in range(70)]), (128, 64, 8, [1] * 63 + [9], [400] * 64),
+    (128, 4, 1, [1] * 5 + [40], [3000] * 6), (256, 8, 8, [1, 1, 1], [2500, 1, 700]), (256, 2, 1, [7] * 9, [333] * 9),
+], ids=str)
+def test_attention_stays_in_its_workspace(dim, heads, kv, rows, lens):
+    """One workspace for calls of all shapes, with memory behind it that must
+    stay; what calls before left in it does not matter."""
+    torch = torch_cuda()
+    gen = np.random.default_rng(dim + len(rows))
+    c = _filled(gen, dim, kv, lens)
+    st, n = _starts(rows), sum(rows)
+    q = _dev(2 * gen.standard_normal((n, heads * dim)).astype(np.float32))
+    s, l = _i32(st), _i32(lens)
+    size = c.dev.kv4_attention_work_bytes(c.c, kv, 1, 1, 1)
+    outs = []
+    for fill in (0xFF, 0x3C):
+        work = torch.full((size + 65536,), fill, dtype=torch.uint8, device="cuda")
+        out, lse = torch.full((n, heads * dim), 7.0, device="cuda"), torch.full((n, heads), 7.0, device="cuda")
+        c.dev.kv4_attention(c.c, aa.F32, q.data_ptr(), heads * dim, heads, n, len(lens), s.data_ptr(), max(rows),
+                            l.data_ptr(), dim ** -0.5, out.data_ptr(), heads * dim, work.data_ptr(), stream(),
+                            lse=lse.data_ptr())
+        sync()
+        assert (work[size:] == fill).all()
+        outs.append((out, lse))
+    _check(c, aa.F32, q, st, lens, heads, dim ** -0.5, 0, *outs[0])
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])

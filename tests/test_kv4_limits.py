@@ -1,0 +1,17 @@
+"""CPU checks of the 4-bit cache calls at the edges of what they allow."""
+import pytest
+
+import aspida_amd as aa
+
+P16 = 1 << 20  # an address that is never followed
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_one_attention_workspace_serves_every_call(dim):
+    """Two parts of 16 columns of 4 dim + 8 bytes for each workgroup that the
+    card holds at once, whatever the rows and sequences."""
+    dev, c = aa.DeviceOps(), aa.KV4Cache(dim, 8, 4, 3, P16, P16)
+    want = 2 * {64: 768, 128: 512, 256: 256}[dim] * 16 * (4 * dim + 8)
+    for args in ((32, 1, 1, 1), (64, 64, 64, 1), (64, 9000, 3, 4097), (64, 9000, 3, 2 ** 31 - 1), (32, 32768, 1, 32768),
+                 (64, 65536, 16, 4096), (64, 4159, 64, 4096), (64, 263, 64, 200), (65528, 2 ** 31 - 1, 65535, 2 ** 31 - 1)):
+        assert dev.kv4_attention_work_bytes(c, *args) == want
