@@ -451,10 +451,9 @@ __global__ __launch_bounds__(256) void kv4_attn_join(SplitArgs s) {
     s.a.lse[(size_t)row * s.a.n_heads + head] = l != 0.f ? (ref + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
 }
 
-// (kv4_prefill_takes leaves at most 1280 + n_kv tiles of all kv heads, or five
-// of each.)
+// (kv4_prefill_takes leaves at most 65535 of all kv heads.)
 static int attn_tiles(int group, int max_rows) {
-  return (int)std::min<long long>(65535, ((long long)max_rows * group + 15) / 16);
+  return (int)(((long long)max_rows * group + 15) / 16);
 }
 // Workgroups that share the axis, of each kv head and column tile.
 template <int D> static int attn_groups(int per_seq) { return std::max(1, ATTN_GROUPS<D> / per_seq); }

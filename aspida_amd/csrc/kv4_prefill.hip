@@ -207,11 +207,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(Pr
   extern __shared__ uint8_t lds[];  // three stages, and the low plane of Q
   const int lane = threadIdx.x & 63, col = lane & 31, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int hk = blockIdx.x, b = blockIdx.z;
+  const int hk = blockIdx.x % s.c.n_kv, b = blockIdx.z;
   const Kv4Span sp = kv4_span(s.rows, b);
   const int n = sp.r1 - sp.r0, nr = min(n, s.a.max_rows);
   // The last rows, which see most, come first.
-  const int tiles = (int)(((long long)nr * s.group + COLS - 1) / COLS), tile = tiles - 1 - (int)blockIdx.y;
+  const int tiles = (int)(((long long)nr * s.group + COLS - 1) / COLS), tile = tiles - 1 - (int)(blockIdx.x / s.c.n_kv);
   if (tile < 0) return;
   const int c0 = tile * COLS, c1 = min(c0 + COLS, nr * s.group);  // the workgroup's columns
   const int first = sp.len - n;                                   // slot of row 0
@@ -467,7 +467,9 @@ static hipError_t prefill_go(const PrefillArgs& s, hipStream_t st) {
                                            hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) return e;
   const long long tiles = ((long long)std::min(s.a.max_rows, s.rows.n_rows) * s.group + 32 * WAVES - 1) / (32 * WAVES);
-  const dim3 grid(s.c.n_kv, (unsigned)tiles, s.rows.n_seq);
+  // Tiles and kv heads share x.  (Its limit is 2^32 threads, 300 GB of queries.)
+  if (tiles * s.c.n_kv >= (1ll << 32) / (64 * WAVES)) return hipErrorInvalidConfiguration;
+  const dim3 grid((unsigned)(tiles * s.c.n_kv), 1, s.rows.n_seq);
   hipLaunchKernelGGL((kv4_prefill<D, T, WAVES>), grid, dim3(64 * WAVES), lds, st, s);
   return hipGetLastError();
 }
@@ -488,9 +490,10 @@ static hipError_t prefill_typed(int head_dim, const PrefillArgs& s, hipStream_t 
 //   and 372 (f32 96: 389 and 409; heads of 256 48: 201 and 194);
 //   rows x heads in all (20000 slots, bf16): 12288 here 679 us, split 400;
 //   24576: 681 and 787 (f32 1066 and 925; heads of 256 12288: 1133 and 813).
+// What the split kernel's launch has no room for comes here in any case.
 bool kv4_prefill_takes(const Kv4View& c, const Kv4Rows& rows, const Kv4Attn& a) {
   const long long cols = (long long)std::min(a.max_rows, rows.n_rows) * (a.n_heads / c.n_kv);
-  return cols >= 80 && (cols + 255) / 256 <= 65535 && (long long)rows.n_rows * a.n_heads >= 20480;
+  return (cols + 15) / 16 * c.n_kv > 65535 || (cols >= 80 && (long long)rows.n_rows * a.n_heads >= 20480);
 }
 
 hipError_t launch_kv4_prefill(int head_dim, const Kv4View& c, int type, const Kv4Rows& rows, const Kv4Attn& a,

@@ -4,7 +4,7 @@ import pytest
 
 import aspida_amd as aa
 from gpu_helpers import stream, sync, torch_cuda
-from test_gpu_kv4 import Cache, _attend, _check, _dev, _filled, _host, _i32, _starts
+from test_gpu_kv4 import HALF, Cache, _attend, _check, _dev, _filled, _host, _i32, _starts, _t
 
 pytestmark = pytest.mark.gpu
 
@@ -82,7 +82,7 @@ def test_windows_beyond_every_slot_hide_nothing(rows, many):
 @pytest.mark.parametrize("dim,heads,kv,rows,lens", [
     (64, 4, 1, [1], [9001]), (64, 64, 8, [1] * 70, [(131 * i) % 900 for i in range(70)]), (128, 64, 8, [1] * 63 + [9], [400] * 64),
     (128, 4, 1, [1] * 5 + [40], [3000] * 6), (256, 8, 8, [1, 1, 1], [2500, 1, 700]), (256, 2, 1, [7] * 9, [333] * 9),
-], ids=str)
+], ids=lambda v: str(v) if isinstance(v, int) else f"{len(v)}x{max(v)}")
 def test_attention_stays_in_its_workspace(dim, heads, kv, rows, lens):
     """One workspace for calls of all shapes, with memory behind it that must
     stay; what calls before left in it does not matter."""
@@ -105,3 +105,34 @@ def test_attention_stays_in_its_workspace(dim, heads, kv, rows, lens):
         outs.append((out, lse))
     _check(c, aa.F32, q, st, lens, heads, dim ** -0.5, 0, *outs[0])
     assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+
+
+@pytest.mark.parametrize("rows,heads,kv,ty", [(131073, 128, 1, aa.BF16), (79, 16384, 16384, aa.F32), (5, 65535, 65535, aa.F16)],
+                         ids=["one_kv_head", "kv_heads", "few_rows"])
+def test_attention_of_more_columns_than_a_launch_of_column_tiles(rows, heads, kv, ty):
+    """Every row of millions of columns is written: with a window of one slot
+    each is the value at its own slot."""
+    torch = torch_cuda()
+    dim, pages = 64, -(-rows // 64)
+    c = Cache(np.random.default_rng(1), dim, kv, 1, pages, spare=0, fill=0)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    k, v = (torch.randn(rows, kv, dim, device="cuda", generator=gen) for _ in range(2))
+    c.append(aa.F32, k, v, [0, rows], [rows])
+    s, l = _i32([0, rows]), _i32([rows])
+    c.dev.kv4_read(c.c, aa.F32, rows, 1, s.data_ptr(), l.data_ptr(), k.data_ptr(), kv * dim, v.data_ptr(), kv * dim, stream())
+    q = torch.randn(rows, heads, dim, device="cuda", generator=gen, dtype=_t(ty))
+    out, lse = torch.full_like(q, 777.0), torch.full((rows, heads), 777.0, device="cuda")
+    work = torch.empty(c.dev.kv4_attention_work_bytes(c.c, heads, rows, 1, rows), dtype=torch.uint8, device="cuda")
+    c.dev.kv4_attention(c.c, ty, q.data_ptr(), heads * dim, heads, rows, 1, s.data_ptr(), rows, l.data_ptr(), 0.125,
+                        out.data_ptr(), heads * dim, work.data_ptr(), stream(), window=1, lse=lse.data_ptr())
+    sync()
+    for a in range(0, rows, 8192):
+        b = min(rows, a + 8192)
+        want = v[a:b].repeat_interleave(heads // kv, 1)
+        # One weight of 1: both its f16 numbers, and the code's and the
+        # minimum's part of at most 16 each, a few roundings of 2^-22.
+        assert ((out[a:b].float() - want).abs() <= HALF[ty] * want.abs() * (1 + 2.0 ** -10) + 2.0 ** -16).all()
+        score = (q[a:b].float() * k[a:b].repeat_interleave(heads // kv, 1)).sum(-1) * 0.125
+        assert ((lse[a:b] - score).abs() <= 2.0 ** -14).all()
+    del c, k, v, q, out, lse
+    torch.cuda.empty_cache()
