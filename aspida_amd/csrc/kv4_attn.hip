@@ -10,7 +10,7 @@
 //   S[token][col] = K Q^T   16x16x32, K's codes as exact f16 (kv4_mma.h), one
 //                           more step for the minima; two planes of Q for f32
 //   P = exp2(S - ref)       ref follows the running maximum per column, moved
-//                           only when a score passes it by 2^8
+//                           only when a score passes it by 15
 //   O[dim][col] += V^T P    P in S's own registers: S's lane holds tokens 4 rg
 //                           + 0..3 of two tiles for one column, which is how
 //                           the value dwords are ordered; one more step for
@@ -272,9 +272,12 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, D == 64 ? 3 : D == 128 ? 2 : 1) vo
         u = 1.f;
       }
       float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * u;
-      if (__ballot(top > ref + 15.f)) {
+      if (__ballot(top > kv4_limit(ref))) {
         // P' = exp2(x - ref) is kept below 2^15; after a move the maximum of the
-        // column is at 2^7.
+        // column is at 2^7.  Large scores are rounded before ref is taken off.
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] *= u;
+        u = 1.f;
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         const float next = fmaxf(ref, top - 7.f);

@@ -45,6 +45,13 @@ __device__ __forceinline__ kvh8 kv4_unpack1(uint32_t w, kvh2 d2) {
   return kv4_unpack(w, d2, d2, d2, d2, n16, n256, n16, n256);
 }
 
+// The score up to which exp2(c u - ref), its product not rounded, is sure to
+// stay below 2^16 and so in f16: ref + 15 while products round by 1/4 at most.
+// Beyond that none is: the product is rounded first, as the maximum was.
+__device__ __forceinline__ float kv4_limit(float ref) {
+  return __builtin_fabsf(ref) < 0x1p22f ? ref + 15.f : -__builtin_inff();
+}
+
 // The page ids of a sequence, 64 at a time in a wave's lanes: a lookup in a
 // loop is a lane read, where a scalar load would make every LDS wait of the
 // loop wait for it too.  Wave-uniform arguments.

@@ -5,7 +5,7 @@
 // turn a stage's codes into f16 operands in LDS once (exact, kv4_mma.h), in
 // the order the 32x32x16 instructions read them, two stages ahead; per stage
 //   S[token][col] = K Q^T      D / 16 steps, and one for the minima
-//   P = exp2(S - ref)          ref moves when a score passes it by 2^15
+//   P = exp2(S - ref)          ref moves when a score passes it by 15
 //   O[dim][col] += V^T P       P in S's own registers: the steps' token order
 //                              is the one in which S's lanes hold them
 //   M[g][col] += m^T P         the minima, with a row of ones that sums P
@@ -354,7 +354,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void kv4_prefill(Pr
 #pragma unroll
     for (int i = 1; i < 16; ++i) top = fmaxf(top, c[i]);
     top *= u;
-    if (__ballot(top > ref + 15.f)) {
+    if (__ballot(top > kv4_limit(ref))) {
+      // (Large scores are rounded before ref is taken off.)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) c[i] *= u;
+      u = 1.f;
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       const float next = fmaxf(ref, top - 7.f), f = __builtin_amdgcn_exp2f(ref - next);
       ref = next;

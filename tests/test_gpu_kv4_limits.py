@@ -4,7 +4,7 @@ import pytest
 
 import aspida_amd as aa
 from gpu_helpers import stream, sync, torch_cuda
-from test_gpu_kv4 import HALF, Cache, _attend, _check, _dev, _filled, _host, _i32, _starts, _t
+from test_gpu_kv4 import HALF, NAMES, Cache, _attend, _check, _dev, _filled, _host, _i32, _starts, _t
 
 pytestmark = pytest.mark.gpu
 
@@ -136,3 +136,31 @@ def test_attention_of_more_columns_than_a_launch_of_column_tiles(rows, heads, kv
         assert ((lse[a:b] - score).abs() <= 2.0 ** -14).all()
     del c, k, v, q, out, lse
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("rows,many", [(3, False), (90, True)], ids=["few", "many"])
+@pytest.mark.parametrize("bits", [10, 18, 22, 24, 26, 28, 30])
+@pytest.mark.parametrize("ty", [aa.F32, aa.BF16], ids=NAMES.get)
+def test_attention_of_scores_of_any_size(ty, bits, rows, many):
+    """Scores around +-2^bits, where f32 holds fewer and fewer of the steps
+    between them: values that are all alike come out whatever the weights."""
+    gen = np.random.default_rng(bits)
+    dim, heads, kv, n = 64, 4, 1, 700
+    k = np.zeros((n, kv, dim), np.float32)
+    k[..., :32] = 1024.0                                           # a constant group, times 32 equal queries
+    k[..., 32:] = np.sort(gen.integers(0, 16, (n, 1, 1)), 0)       # steps of 1 between the slots' scores
+    k[..., 32], k[..., 33] = 0, 15
+    v = np.repeat(gen.standard_normal((1, kv, dim)), n, 0).astype(np.float32)
+    c = Cache(gen, dim, kv, 1, 11)
+    c.append(aa.F32, _dev(k), _dev(v), [0, n], [n])
+    value = c.all([n])[0][1][0, 0]
+    for sign in (1, -1):
+        q = np.zeros((rows, heads, dim), np.float32)
+        q[..., :32] = sign * 2.0 ** (bits - 15)
+        q[..., 34] = 1
+        out, lse = _attend(c, ty, _dev(q.reshape(rows, -1), ty), [0, rows], [n], heads, 1.0, many=many)
+        off = np.abs(_host(out).reshape(-1, dim) - value)
+        # One value times the sum of all weights over the same sum.
+        assert np.all(off <= HALF[ty] * np.abs(value) * (1 + 2.0 ** -10) + 2.0 ** -16)
+        # Between the largest score and that of all slots: 15 + log 700; sums of 2^bits in f32.
+        assert np.all(np.abs(_host(lse) - sign * 2.0 ** bits) <= 22 + 2.0 ** (bits - 19))
