@@ -373,7 +373,7 @@ class DeviceOps:
 
     def rope(self, rope, type, x, x_stride, n_tok, n_heads, head_dim, pos, y, y_stride, stream=0, inverse=False):
         """y = x [n_tok][n_heads][head_dim] rotated to pos (a ``Rope``; inverse turns back)."""
-        self._ok(self.lib.aspida_rope_dev(rope.h, type, x, x_stride, n_tok, n_heads, head_dim, pos,
+        self._ok(self.lib.aspida_rope_dev(rope.handle(), type, x, x_stride, n_tok, n_heads, head_dim, pos,
                                           1 if inverse else 0, y, y_stride, stream), "aspida_rope_dev")
 
     def kv4_page_bytes(self, head_dim, n_kv):
@@ -383,7 +383,7 @@ class DeviceOps:
                    stream=0):
         """Write key and value rows into a ``KV4Cache``, keys rotated to pos by rope (None: as they are)."""
         self._ok(self.lib.aspida_kv4_append_dev(cache.ref, type, k, k_stride, v, v_stride, n_rows, n_seq, row_start,
-                                                kv_len, rope.h if rope else None, pos, stream),
+                                                kv_len, rope.handle() if rope else None, pos, stream),
                  "aspida_kv4_append_dev")
 
     def kv4_read(self, cache, type, n_rows, n_seq, row_start, kv_len, k, k_stride, v, v_stride, stream=0):
@@ -470,10 +470,15 @@ class Rope:
         if not self.h:
             raise RuntimeError(f"aspida_rope_create failed (error {self.lib.aspida_gpu_last_error()})")
 
+    def handle(self):
+        if not self.h:
+            raise ValueError("Rope: closed")
+        return self.h
+
     def table(self):
         """(angle per position of each pair, multiplier)."""
         f, m = np.empty(self.rot_dim // 2), ctypes.c_double()
-        self.lib.aspida_rope_table(self.h, _p(f), ctypes.byref(m))
+        self.lib.aspida_rope_table(self.handle(), _p(f), ctypes.byref(m))
         return f, m.value
 
     def close(self):

@@ -15,3 +15,15 @@ def test_one_attention_workspace_serves_every_call(dim):
     for args in ((32, 1, 1, 1), (64, 64, 64, 1), (64, 9000, 3, 4097), (64, 9000, 3, 2 ** 31 - 1), (32, 32768, 1, 32768),
                  (64, 65536, 16, 4096), (64, 4159, 64, 4096), (64, 263, 64, 200), (65528, 2 ** 31 - 1, 65535, 2 ** 31 - 1)):
         assert dev.kv4_attention_work_bytes(c, *args) == want
+
+
+def test_a_closed_rotation_is_refused():
+    """Also where no rotation is a choice: keys are not stored unrotated by mistake."""
+    dev, c, rope = aa.DeviceOps(), aa.KV4Cache(128, 2, 4, 3, P16, P16), aa.Rope(64)
+    rope.close()
+    with pytest.raises(ValueError):
+        rope.table()
+    with pytest.raises(ValueError):
+        dev.rope(rope, aa.F32, P16, 256, 0, 2, 128, P16, P16, 256)
+    with pytest.raises(ValueError):
+        dev.kv4_append(c, aa.F32, P16, 256, P16, 256, 0, 0, 0, P16, rope, P16)  # no rows: nothing is followed
