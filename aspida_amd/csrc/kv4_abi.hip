@@ -111,6 +111,10 @@ extern "C" void* aspida_rope_create(const aspida_rope_params* p) {
       const double ramp = std::fmin(1.0, std::fmax(0.0, (i - lo) / std::fmax(hi - lo, 0.001)));
       f = f / p->factor * ramp + f * (1.0 - ramp);
     }
+    if (!(f <= kq::ROPE_MAX_FREQ)) {
+      delete t;
+      return bad("aspida_rope_create: a pair turns by more than 2^19 a position");
+    }
     t->freq[i] = f;
   }
   t->mag = p->magnitude > 0.0 ? p->magnitude : p->scaling == 3 ? 0.1 * std::log(p->factor) + 1.0 : 1.0;

@@ -11,6 +11,7 @@
 namespace kq {
 
 constexpr int ROPE_MAX_ROT = 256;
+constexpr double ROPE_MAX_FREQ = 524288.0;  // |pos f| <= 2^50, as sincos_f64 needs
 
 // Passed to the kernels by value (1 KB of arguments), so a captured graph
 // holds the table itself and no device memory belongs to a rotation.
@@ -33,10 +34,11 @@ typedef __bf16 bf16_t;
 
 template <class T> __device__ __forceinline__ float act_f32(T v) { return (float)v; }
 
-// sin and cos of theta to about an ulp of f64 for |theta| < 2^31: theta less
+// sin and cos of theta to about an ulp of f64 for |theta| <= 2^50: theta less
 // the nearest multiple n of pi/2 in two fma steps (pi/2 as a sum of two f64;
-// n times what a third would add is below 2^-70), then the Taylor series at
-// |r| <= pi/4, whose first dropped terms are r^19/19! and r^18/18! (< 2^-58).
+// n times what a third would add is below 2^-59), then the Taylor series at
+// |r| <= pi/4 (0.86 at 2^50, where n may be the second nearest), whose first
+// dropped terms are r^19/19! and r^18/18! (below 2^-56).
 __device__ __forceinline__ void sincos_f64(double theta, double& s, double& c) {
   // n + 1.5 2^52 has n's low bits at the end of its significand.
   const double at = __builtin_fma(theta, 0.63661977236758134308, 6755399441055744.0);

@@ -240,6 +240,7 @@ int aspida_moe_experts_packed_dev(const float *x, int T, int dim, int top_k, int
 
 /* A rotation: pair i of a head's first rot_dim values (even, 2 to 256) turns
  * by pos * f_i, f_i = base^(-2 i / rot_dim); the angle is formed in f64.
+ * After freq_factors and scaling f_i must be at most 2^19.
  * Pairs are (i, i + rot_dim / 2), or (2 i, 2 i + 1) when interleaved; the
  * values behind rot_dim pass through.  freq_factors (host, rot_dim / 2 values
  * as in a GGUF rope_freqs.weight, or NULL) divide f first.  scaling:

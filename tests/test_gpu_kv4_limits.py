@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 
 import aspida_amd as aa
+import kv4_plain as plain
 from gpu_helpers import stream, sync, torch_cuda
 from test_gpu_kv4 import HALF, NAMES, Cache, _attend, _check, _dev, _filled, _host, _i32, _starts, _t
 
@@ -164,3 +165,22 @@ def test_attention_of_scores_of_any_size(ty, bits, rows, many):
         assert np.all(off <= HALF[ty] * np.abs(value) * (1 + 2.0 ** -10) + 2.0 ** -16)
         # Between the largest score and that of all slots: 15 + log 700; sums of 2^bits in f32.
         assert np.all(np.abs(_host(lse) - sign * 2.0 ** bits) <= 22 + 2.0 ** (bits - 19))
+
+
+@pytest.mark.parametrize("factor", [1.0, 2.0 ** -10, 2.0 ** -19])
+def test_rope_at_the_largest_angles(factor):
+    """Positions up to the ends of int, angles up to 2^50."""
+    torch = torch_cuda()
+    gen = np.random.default_rng(8)
+    pos = np.concatenate([[-2 ** 31, 2 ** 31 - 1, -1, 0, 1], gen.integers(-2 ** 31, 2 ** 31, 1000)])
+    rope = aa.Rope(8, base=3.0, scaling="linear", factor=factor)
+    f, mag = rope.table()
+    x = gen.standard_normal((len(pos), 1, 8)).astype(np.float32)
+    dx, dp = _dev(x), _i32(pos)
+    y = torch.empty_like(dx)
+    aa.DeviceOps().rope(rope, aa.F32, dx.data_ptr(), 8, len(pos), 1, 8, dp.data_ptr(), y.data_ptr(), 8, stream())
+    sync()
+    want = plain.rotate(x, pos, f, mag, False)
+    # cos, sin, two products and the result round by half a step of f32 each.
+    size = np.tile(np.abs(x[..., :4]) + np.abs(x[..., 4:]), 2)
+    assert np.all(np.abs(_host(y) - want) <= 4 * HALF[aa.F32] * size + HALF[aa.F32] * np.abs(want))

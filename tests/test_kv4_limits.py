@@ -27,3 +27,16 @@ def test_a_closed_rotation_is_refused():
         dev.rope(rope, aa.F32, P16, 256, 0, 2, 128, P16, P16, 256)
     with pytest.raises(ValueError):
         dev.kv4_append(c, aa.F32, P16, 256, P16, 256, 0, 0, 0, P16, rope, P16)  # no rows: nothing is followed
+
+
+@pytest.mark.parametrize("kw", [dict(freq_factors=[1e-30, 1.0]), dict(freq_factors=[1.0, 1e-12]),
+                                dict(scaling="linear", factor=2.0 ** -19 * 0.999), dict(scaling="linear", factor=1e-300),
+                                dict(scaling="yarn", factor=1e-9, low=1.0, high=32.0, context=4096)], ids=str)
+def test_rotations_too_fast_for_their_angles_are_refused(kw):
+    with pytest.raises(RuntimeError):
+        aa.Rope(4, **kw)
+    assert aa.load().aspida_gpu_last_error() == 0  # the constructor took it
+
+
+def test_the_fastest_rotation():
+    assert aa.Rope(4, scaling="linear", factor=2.0 ** -19).table()[0][0] == 2.0 ** 19
