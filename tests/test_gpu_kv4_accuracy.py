@@ -7,7 +7,8 @@ import pytest
 import aspida_amd as aa
 import kv4_accuracy as acc
 import kv4_plain as plain
-from test_gpu_kv4 import NAMES, Cache, _attend, _check, _dev, _filled, _host, _kv, _starts
+from gpu_helpers import stream, sync, torch_cuda
+from test_gpu_kv4 import NAMES, Cache, _attend, _check, _dev, _filled, _host, _i32, _kv, _starts
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +74,42 @@ def test_attention_of_values_at_the_ends_of_f16(dim, ty, rows, many):
         hq = _host(q).reshape(rows, heads, dim)
         want = plain.attend(hq, *kvs[0], scale)[0]
         assert acc.over(_host(out).reshape(want.shape), want, acc.attend32(hq, *kvs[0], scale)[0]) <= 1
+
+
+@pytest.mark.parametrize("ty", [aa.F32, aa.BF16, aa.F16], ids=NAMES.get)
+@pytest.mark.parametrize("scale", [1.0, -1.0], ids=["plus", "minus"])
+@pytest.mark.parametrize("case", [
+    (128, 32, 8, [1] * 6, [3000, 65, 700, 1000, 33, 512], 0),
+    (64, 8, 2, [3, 2, 3], [700, 1300, 90], 0),
+    (256, 8, 4, [2, 2], [500, 301], 100),
+    (128, 8, 2, [40, 31], [400, 900], 0),
+    (64, 8, 2, [90], [777], 0),
+    (256, 8, 4, [20, 1], [600, 70], 200),
+], ids=lambda c: f"d{c[0]}r{c[3][0]}")
+def test_slot_weights_are_as_accurate_as_f32(case, scale, ty):
+    """Each slot's weight, for negative scales and query rows at an odd stride too."""
+    dim, heads, kv, rows, lens, window = case
+    torch = torch_cuda()
+    gen = np.random.default_rng(dim + heads + sum(lens))
+    c = _filled(gen, dim, kv, lens)
+    st, scale = _starts(rows), scale * dim ** -0.5
+    wide = heads * dim + 3
+    q = _dev(2 * gen.standard_normal((st[-1], wide)).astype(np.float32), ty)
+    _, lse = _attend(c, ty, q, st, lens, heads, scale, window)
+    stride = max(lens)
+    out = torch.full((len(lens), kv, stride), 7.0, device="cuda")
+    s, l = _i32(st), _i32(lens)
+    c.dev.kv4_weigh(c.c, ty, q.data_ptr(), wide, heads, int(st[-1]), len(lens), s.data_ptr(), max(rows), l.data_ptr(),
+                    scale, lse.data_ptr(), 0, out.data_ptr(), stride, stream(), window=window)
+    sync()
+    got, hl, hq = _host(out), _host(lse), _host(q)[:, :heads * dim].reshape(-1, heads, dim)
+    ratio, ratio32 = [], []
+    for b, (k, v) in enumerate(c.all(lens)):
+        r, n = slice(st[b], st[b + 1]), lens[b]
+        want = plain.weights(hq[r], k, hl[r], scale, window)
+        w32 = acc.weights32(hq[r], k, hl[r], scale, window)
+        assert (got[b][:, n:] == 0).all() and (got[b][:, :n][want == 0] == 0).all()
+        some = want > 1e-30
+        ratio.append(got[b][:, :n][some] / want[some])
+        ratio32.append(w32[some] / want[some])
+    assert acc.over(np.concatenate(ratio), 1.0, np.concatenate(ratio32)) <= 1

@@ -184,3 +184,71 @@ def test_rope_at_the_largest_angles(factor):
     # cos, sin, two products and the result round by half a step of f32 each.
     size = np.tile(np.abs(x[..., :4]) + np.abs(x[..., 4:]), 2)
     assert np.all(np.abs(_host(y) - want) <= 4 * HALF[aa.F32] * size + HALF[aa.F32] * np.abs(want))
+
+
+def test_a_prompt_with_weights_and_eviction_captured():
+    """A prompt's chunks (rows behind what is cached), slot weights and an
+    eviction in one graph: replays read lengths, rows and positions anew and
+    give the bits of eager calls, with eager work between them."""
+    torch = torch_cuda()
+    gen = np.random.default_rng(23)
+    dim, heads, kv, n, keep = 128, 16, 2, 700, 200
+    rope = aa.Rope(dim, base=10000.0)
+    src, dst = (Cache(np.random.default_rng(i), dim, kv, 2, p, spare=0, fill=0) for i, p in ((1, 40), (2, 4)))
+    dev, empty = src.dev, lambda *s: torch.empty(*s, device="cuda")  # noqa: E731
+    k, v, q = empty(n, kv, dim), empty(n, kv, dim), empty(n, heads, dim)
+    turned, out, lse = torch.empty_like(q), torch.empty_like(q), empty(n, heads)
+    acc, kept, idx = empty(2, kv, 2560), empty(2, kv, keep), torch.empty(2, kv, keep, dtype=torch.int32, device="cuda")
+    starts, lens, new, pos = _i32([0, 1, n]), _i32([0, 0]), _i32([0, 0]), _i32(np.zeros(n))
+    work = torch.empty(dev.kv4_attention_work_bytes(src.c, heads, n, 2, n), dtype=torch.uint8, device="cuda")
+    few = torch.empty_like(out)
+
+    def run():
+        sp, row = stream(), kv * dim
+        dev.kv4_append(src.c, aa.F32, k.data_ptr(), row, v.data_ptr(), row, n, 2, starts.data_ptr(), lens.data_ptr(), rope,
+                       pos.data_ptr(), sp)
+        dev.rope(rope, aa.F32, q.data_ptr(), heads * dim, n, heads, dim, pos.data_ptr(), turned.data_ptr(), heads * dim, sp)
+        for rows, o in ((n, out), (8, few)):  # the kernel of many rows, and that of few (rows past 8 are NaN)
+            m = n if rows == n else 12
+            dev.kv4_attention(src.c, aa.F32, turned.data_ptr(), heads * dim, heads, m, 2, starts.data_ptr(), rows,
+                              lens.data_ptr(), dim ** -0.5, o.data_ptr(), heads * dim, work.data_ptr(), sp,
+                              lse=lse.data_ptr() if rows == n else 0)
+        dev.kv4_weigh(src.c, aa.F32, turned.data_ptr(), heads * dim, heads, n, 2, starts.data_ptr(), n, lens.data_ptr(),
+                      dim ** -0.5, lse.data_ptr(), 0, acc.data_ptr(), 2560, sp)
+        dev.kv4_evict(src.c, 2, lens.data_ptr(), acc.data_ptr(), 2560, keep, 4, 32, dst.c, new.data_ptr(), idx.data_ptr(),
+                      kept.data_ptr(), sp)
+
+    def turns(call):
+        got = []
+        for i, (split, before) in enumerate(((1, (0, 0)), (350, (1, 699)), (650, (351, 1049)))):
+            g = torch.Generator(device="cuda").manual_seed(i)
+            for x in (k, v, q):
+                x.copy_(torch.randn(x.shape, device="cuda", generator=g))
+            starts.copy_(_i32([0, split, n]))
+            lens.copy_(_i32([before[0] + split, before[1] + n - split]))
+            pos.copy_(torch.cat([torch.arange(split, device="cuda") + before[0],
+                                 torch.arange(n - split, device="cuda") + before[1]]).int())
+            few.zero_()
+            call()
+            sync()
+            assert torch.isfinite(out).all() and new.cpu().tolist() == [min(int(m), keep) for m in lens.cpu()]
+            got.append([x.clone() for x in (out, lse, few, acc, idx, kept, dst.pages)])
+        return got
+    eager = turns(run)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        run()
+    sync()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        run()
+
+    def replay():
+        graph.replay()
+        torch.ones(1000, device="cuda").sum()
+    for _ in range(2):
+        src.pages.zero_(), dst.pages.zero_()
+        for a, b in zip(eager, turns(replay)):
+            for x, y in zip(a, b):
+                assert torch.equal(x.nan_to_num(123.0) if x.is_floating_point() else x,
+                                   y.nan_to_num(123.0) if y.is_floating_point() else y)
