@@ -25,9 +25,10 @@
 // lengths on the device, which the host does not know.
 // Bound by the vector units: a wave's round of 32 tokens is about 300 of their
 // instructions (unpacking, exp2, the two planes of P) in 1800 cycles, with
-// two waves a SIMD, and 45 matrix instructions beside them.  130001 slots of 8
-// kv heads of 128 (f32, 166 MB) take 42 us, 4.0 TB/s, of 32 at the rate of a
-// large copy; 64 lanes of up to 8000 slots (bf16, 330 MB) 79 us, 4.2 TB/s.
+// two waves a SIMD, and 45 matrix instructions beside them (64 lanes: vector
+// units 73% busy, matrix cores 18%).  130001 slots of 8 kv heads of 128 (f32,
+// 166 MB) take 42 us, 4.0 TB/s, of 32 at the rate of a large copy; 64 lanes of
+// up to 8000 slots (bf16, 330 MB) 79 us, 4.2 TB/s.
 #include <algorithm>
 
 #include "kv4_mma.h"

@@ -123,10 +123,11 @@ __device__ __forceinline__ uint32_t kv4_put(uint32_t w, uint32_t q, int j) {
 // eight tokens.
 // One loop body serves values and keys, the next group's loads ahead of it
 // (unrolled, 20 KB of code for a few rounds).  Frequencies go through LDS:
-// arguments are far memory, and prompts of 6500 rows in all of 8 heads of 128
-// (bf16) took 57 us with each pair's read from there, 34 now.  Bound by its
-// sums (66% of the issue slots; without the angles 24 us), copies of the same
-// bytes take 7.
+// arguments are far memory, and prompts of 7352 rows in all of 8 heads of 128
+// (bf16) took 57 us with each pair's read from there, 34 now.  Bound by the
+// vector units (77% of a busy unit's issue slots; without the angles, which
+// each of the four workgroups of two heads forms anew, 24 us), copies of the
+// same bytes take 8.  A single row passes through the body made for 32.
 // How keys are rotated: not; values 8 i .. 8 i + 7 with others of that kind
 // (half layout, rot_dim a multiple of 16); in any other way.
 enum : int { ROPE_NONE, ROPE_EIGHTS, ROPE_ANY };
@@ -361,7 +362,7 @@ template <int D, class T>
 static void append_go(const AppendArgs& a, bool rope, hipStream_t s) {
   const unsigned blocks = blocks_of(a.rows, a.c.n_kv);
   // Heads a workgroup takes in turn, as far as that leaves three workgroups a
-  // compute unit (6500 rows of 8 heads: one 34.7 us, two 33.8).
+  // compute unit (7352 rows of 8 heads: one 34.7 us, two 33.8).
   const long long all = ((long long)a.rows.n_rows / 32 + a.rows.n_seq) * a.c.n_kv;
   const int turns = rope ? (int)std::min<long long>(std::max<long long>(all / 768, 1), a.c.n_kv) : 1;
   const dim3 grid(blocks, (a.c.n_kv + turns - 1) / turns, a.rows.n_seq);

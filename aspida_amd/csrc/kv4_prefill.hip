@@ -15,14 +15,15 @@
 // of m): the sums over thousands of slots then stay near the result instead of
 // cancelling against the minima (6000 slots: error 3.1e-6 before, of 1.5e-6 in
 // plain f32).
-// Bound by issue: the matrix cores are busy 37% of the time, the vector units
-// 43% (unpacking, exp2, the planes of P, address sums), LDS 26%, two waves a
-// SIMD in turns.  2000 rows behind 4000 slots (32/8 heads of 128, f32, 328
-// GFLOP of two planes) 385 us, 850 TFLOP/s; prompts up to 4097 rows (bf16,
-// 391 GFLOP and half as many for P's low plane) 672 us, 870 TFLOP/s; a large
-// f16 product reaches 1108.  Measured and not taken: four waves a workgroup,
-// priorities of waves, dwords instead of 16-byte pieces per unpacking thread
-// (with one plane of P 598 us for 557).
+// Bound by waiting: of a busy compute unit's cycles the matrix cores work 51%
+// (f32 60%), the vector units 52% (44%: unpacking, exp2, the planes of P),
+// LDS 30%, and each of the two waves a SIMD waits a third of its time for data
+// and the barrier of every 32 tokens.  2000 rows behind 4000 slots (32/8 heads
+// of 128, f32, 164 GFLOP, twice with both planes) 397 us, 830 TFLOP/s of them;
+// prompts up to 4097 rows (bf16, 391 GFLOP, half as many again for P's low
+// plane) 688 us, 850 TFLOP/s; a large f16 product reaches 1108.  Measured and
+// not taken: four waves a workgroup, priorities of waves, dwords instead of
+// 16-byte pieces per unpacking thread (with one plane of P 598 us for 557).
 #include <algorithm>
 
 #include "kv4_mma.h"
@@ -490,10 +491,18 @@ static hipError_t prefill_typed(int head_dim, const PrefillArgs& s, hipStream_t 
 // per 16 columns.  So this one is for sequences of many columns, and for
 // enough of them in all that most compute units have some:
 //   columns of a (sequence, kv head), card full (64 sequences of 3000 slots,
-//   32/8 heads, bf16): 48 here 241 us, split 194; 64: 243 and 223; 96: 246
-//   and 372 (f32 96: 389 and 409; heads of 256 48: 201 and 194);
-//   rows x heads in all (20000 slots, bf16): 12288 here 679 us, split 400;
-//   24576: 681 and 787 (f32 1066 and 925; heads of 256 12288: 1133 and 813).
+//   32/8 heads, bf16): 48 here 287 us, split 207; 64: 285 and 227; 80: 300 and
+//   305; 96: 299 and 383 (f32 80: 386 and 317; 96: 383 and 400; heads of 256,
+//   80: 253 and 319; of 64, 80: 226 and 208);
+//   rows x heads in all (six sequences, 20000 slots, bf16): 12288 here 819 us,
+//   split 447; 18432: 816 and 805; 24576: 820 and 822; 30720: 823 and 1610
+//   (f32 24576: 1130 and 869; 30720: 1127 and 1673; heads of 64, 24576: 691
+//   and 563; of 256, 24576: 1469 and 1701).
+// All of it for sequences alike.  A sequence of a few rows beside a long one
+// goes where that one does: its slots are not cut here, and there fewer
+// workgroups share the axis (64/8 heads, bf16: 63 lanes of up to 8000 slots 94
+// us and 200 rows 39, together 2630; a lane of 130001 slots 42 and 2000 rows
+// 146, together 5120).
 // What the split kernel's launch has no room for comes here in any case.
 bool kv4_prefill_takes(const Kv4View& c, const Kv4Rows& rows, const Kv4Attn& a) {
   const long long cols = (long long)std::min(a.max_rows, rows.n_rows) * (a.n_heads / c.n_kv);

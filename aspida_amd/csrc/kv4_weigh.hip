@@ -11,13 +11,15 @@
 //                   registers, a wave walks pages with the next one in
 //                   flight.  32 lanes of 8 kv heads of 128 (f32, 113 MB) 33
 //                   us, 3.4 TB/s, of 22 at the rate of a large copy: bound
-//                   by the keys' bytes and, half of the time, by unpacking.
-//                   (Loads without a branch, ids a step ahead: 34 us.)
+//                   by the vector units, 74% busy (unpacking, exp2, sums over
+//                   columns).  (Loads without a branch, ids a step ahead: 34.)
 //   kv4_weigh_many  a wave turns its page's keys into operands once; column
 //                   tiles pass through LDS, each made by one wave and used by
 //                   all.  64 rows over 32000 slots (64/8 heads of 128,
 //                   bf16, 33.5 GFLOP) 77 us, of 29 at the rate of a large
-//                   product: bound by exp2 and the sums over columns.
+//                   product.  No unit is full (vector units 53%, matrix
+//                   cores 23%): a tile's operands are read, multiplied, raised
+//                   and summed one after the other, and waves wait 43%.
 #include <algorithm>
 
 #include "kv4_mma.h"
