@@ -87,6 +87,19 @@ def load(path=None):
         "aspida_kv4_attn_dev": (I, [P, I, P, LL, I, I, I, P, I, P, F, I, P, LL, P, P, P]),
         "aspida_kv4_weigh_dev": (I, [P, I, P, LL, I, I, I, P, I, P, F, I, P, P, P, LL, P]),
         "aspida_kv4_evict_dev": (I, [P, I, P, P, LL, I, I, I, P, P, P, P, P]),
+        "aspida_tree_dev": (I, [P, I, I, P, P, P, P, I, P]),
+        "aspida_kv4_tree_attn_work_bytes": (LL, [P, I, I, I, I]),
+        "aspida_kv4_tree_attn_dev": (I, [P, I, P, LL, I, I, I, P, I, P, P, I, F, I, P, LL, P, P, P]),
+        "aspida_tree_accept_work_bytes": (LL, [I, I]),
+        "aspida_tree_accept_dev": (I, [I, P, LL, I, I, I] + [P] * 10),
+        "aspida_kv4_keep_dev": (I, [P, I, I, P, P, P, P, P]),
+        "aspida_w8_bytes": (LL, [I, I]),
+        "aspida_w8_pack_dev": (I, [P, LL, P, I, I, P, P]),
+        "aspida_w8_convert_dev": (I, [I, P, I, I, P, P]),
+        "aspida_w8_unpack_dev": (I, [P, I, I, P, P]),
+        "aspida_w8_work_bytes": (LL, [I, I]),
+        "aspida_w8_matmul_dev": (I, [P, I, I, I, P, LL, I, P, LL, P, P]),
+        "aspida_w8_gated_dev": (I, [P, P, I, I, I, I, P, LL, I, P, LL, P, P]),
         "aspida_kq_chain_create": (P, [P, I]),
         "aspida_kq_chain_run": (I, [P, P]),
         "aspida_kq_chain_check": (I, [P]),
@@ -416,6 +429,77 @@ class DeviceOps:
         self._ok(self.lib.aspida_kv4_evict_dev(src.ref, n_seq, kv_len, acc, acc_stride, keep, first, recent, dst.ref,
                                                new_len, idx, acc_out, stream), "aspida_kv4_evict_dev")
 
+    def tree(self, parent, n_rows, n_seq, row_start, kv_len, pos=0, mask=0, mask_words=0, stream=0):
+        """Positions and ancestor masks (uint32 [n_rows][mask_words]) of trees of drafted tokens, from parents."""
+        self._ok(self.lib.aspida_tree_dev(parent, n_rows, n_seq, row_start, kv_len, pos, mask, mask_words, stream),
+                 "aspida_tree_dev")
+
+    def kv4_tree_attention_work_bytes(self, cache, n_heads, n_rows, n_seq, max_rows):
+        n = int(self.lib.aspida_kv4_tree_attn_work_bytes(cache.ref, n_heads, n_rows, n_seq, max_rows))
+        if n < 0:
+            raise ValueError(f"aspida_kv4_tree_attn_work_bytes: bad arguments ({n_heads}, {n_rows}, {n_seq}, "
+                             f"{max_rows})")
+        return n
+
+    def kv4_tree_attention(self, cache, type, q, q_stride, n_heads, n_rows, n_seq, row_start, max_rows, kv_len, mask,
+                           mask_words, scale, out, out_stride, work, stream=0, window=0, lse=0):
+        """Attention of trees of drafted tokens: slots before the tree, and the rows that each row's mask names."""
+        self._ok(self.lib.aspida_kv4_tree_attn_dev(cache.ref, type, q, q_stride, n_heads, n_rows, n_seq, row_start,
+                                                   max_rows, kv_len, mask, mask_words, scale, window, out, out_stride,
+                                                   lse, work, stream), "aspida_kv4_tree_attn_dev")
+
+    def tree_accept_work_bytes(self, n_rows, vocab):
+        n = int(self.lib.aspida_tree_accept_work_bytes(n_rows, vocab))
+        if n < 0:
+            raise ValueError(f"aspida_tree_accept_work_bytes: bad arguments ({n_rows}, {vocab})")
+        return n
+
+    def tree_accept(self, type, logits, stride, vocab, n_rows, n_seq, row_start, kv_len, parent, token, path, count,
+                    next, new_len, work, stream=0):
+        """The drafted tokens that the logits' greedy choice confirms, from each tree's row 0 on."""
+        self._ok(self.lib.aspida_tree_accept_dev(type, logits, stride, vocab, n_rows, n_seq, row_start, kv_len, parent,
+                                                 token, path, count, next, new_len, work, stream),
+                 "aspida_tree_accept_dev")
+
+    def kv4_keep(self, cache, n_rows, n_seq, row_start, kv_len, path, count, stream=0):
+        """Move the accepted rows of each tree together in a ``KV4Cache``."""
+        self._ok(self.lib.aspida_kv4_keep_dev(cache.ref, n_rows, n_seq, row_start, kv_len, path, count, stream),
+                 "aspida_kv4_keep_dev")
+
+    def _w8_size(self, what, *args):
+        n = int(getattr(self.lib, what)(*args))
+        if n < 0:
+            raise ValueError(f"{what}: bad arguments {args}")
+        return n
+
+    def w8_bytes(self, in_dim, out_dim):
+        return self._w8_size("aspida_w8_bytes", in_dim, out_dim)
+
+    def w8_work_bytes(self, n_rows, in_dim):
+        return self._w8_size("aspida_w8_work_bytes", n_rows, in_dim)
+
+    def w8_pack(self, codes, stride, scale, in_dim, out_dim, packed, stream=0):
+        """Lay out int8 codes [out_dim] rows `stride` apart and f32 scales [out_dim]."""
+        self._ok(self.lib.aspida_w8_pack_dev(codes, stride, scale, in_dim, out_dim, packed, stream),
+                 "aspida_w8_pack_dev")
+
+    def w8_convert(self, kind, w, in_dim, out_dim, packed, stream=0):
+        """Packed 8-bit weights from a matrix of a quantised kind, or of f32 (kind -1)."""
+        self._ok(self.lib.aspida_w8_convert_dev(kind, w, in_dim, out_dim, packed, stream), "aspida_w8_convert_dev")
+
+    def w8_unpack(self, packed, in_dim, out_dim, w, stream=0):
+        self._ok(self.lib.aspida_w8_unpack_dev(packed, in_dim, out_dim, w, stream), "aspida_w8_unpack_dev")
+
+    def w8_matmul(self, packed, in_dim, out_dim, type, x, x_stride, n_rows, y, y_stride, work, stream=0):
+        """y = x W^T with 8-bit integer weights and activations quantised per token."""
+        self._ok(self.lib.aspida_w8_matmul_dev(packed, in_dim, out_dim, type, x, x_stride, n_rows, y, y_stride, work,
+                                               stream), "aspida_w8_matmul_dev")
+
+    def w8_gated(self, gate, up, in_dim, out_dim, act, type, x, x_stride, n_rows, y, y_stride, work, stream=0):
+        """y = act(x gate^T) * (x up^T); act ``SILU`` or ``GELU``."""
+        self._ok(self.lib.aspida_w8_gated_dev(gate, up, in_dim, out_dim, act, type, x, x_stride, n_rows, y, y_stride,
+                                              work, stream), "aspida_w8_gated_dev")
+
     def chain(self, steps):
         """A resident decode chain over steps [(kind, packed_ptr, in_dim, out_dim, x_ptr, y_ptr), ...]."""
         return Chain(self.lib, steps)
@@ -439,6 +523,8 @@ class DeviceOps:
 
 # Activation types of the rotary and cache calls.
 F32, F16, BF16 = 0, 1, 2
+# Activations of the gated feed-forward block.
+SILU, GELU = 0, 1
 
 
 class _RopeParams(ctypes.Structure):

@@ -71,6 +71,10 @@ struct Kv4Attn {
   void* work;
   int n_heads, max_rows, window;
   float scale;
+  // Rows that are a tree: bit j of a row's mask [n_rows][mask_words] says that
+  // it sees its sequence's row j.  Null: a row sees those before it.
+  const uint32_t* mask;
+  int mask_words;
 };
 size_t kv4_attn_work_bytes(int head_dim);
 hipError_t launch_kv4_attn(int head_dim, const Kv4View& c, int type, const Kv4Rows& rows, const Kv4Attn& a,
@@ -104,6 +108,11 @@ struct Kv4Evict {
   float* acc_out;  // [n_seq][n_kv][keep]
 };
 hipError_t launch_kv4_evict(int head_dim, const Kv4View& src, const Kv4View& dst, const Kv4Evict& e, hipStream_t s);
+
+// Slot base + i of a sequence takes what slot base + path[i] holds (i <
+// count[b], base the slot of its row 0).
+hipError_t launch_kv4_keep(int head_dim, const Kv4View& c, const Kv4Rows& rows, const int* path, const int* count,
+                           hipStream_t s);
 
 #ifdef __HIPCC__
 typedef _Float16 kvh2 __attribute__((ext_vector_type(2)));

@@ -1,5 +1,5 @@
-// kv4_abi.hip -- C entry points of the rotary positions and the 4-bit
-// key/value cache (contracts: include/aspidagpu.h).  Arguments that the host
+// kv4_abi.hip -- C entry points of the rotary positions, the 4-bit key/value
+// cache and trees of drafted tokens (contracts: include/aspidagpu.h).  Arguments that the host
 // can see are checked here; lengths, row starts and page ids live on the
 // device and are bounded by the kernels.
 #include <cerrno>
@@ -10,6 +10,7 @@
 
 #include "../../include/aspidagpu.h"
 #include "kv4.h"
+#include "tree.h"
 
 namespace kq {
 void abi_report(int code, const char* what);  // aspidagpu.hip: the calling thread's aspida_gpu_last_error
@@ -201,7 +202,7 @@ extern "C" int aspida_kv4_attn_dev(const aspida_kv4* cache, int type, const void
       !valid_rows(out, type, out_stride, n_heads, cache->head_dim) || (lse && !aligned(lse, 4)) ||
       !aligned(work, 256))
     return -EINVAL;
-  kq::Kv4Attn a{q, q_stride, out, out_stride, lse, work, n_heads, longest(max_rows, n_rows), window, scale};
+  kq::Kv4Attn a{q, q_stride, out, out_stride, lse, work, n_heads, longest(max_rows, n_rows), window, scale, nullptr, 0};
   return done(kq::launch_kv4_attn(cache->head_dim, view(cache), type, r, a, (hipStream_t)stream),
               "aspida_kv4_attn_dev");
 }
@@ -235,4 +236,72 @@ extern "C" int aspida_kv4_evict_dev(const aspida_kv4* src, int n_seq, const int*
   kq::Kv4Evict e{kv_len, acc, acc_stride, n_seq, keep, first, recent, new_len, idx, acc_out};
   return done(kq::launch_kv4_evict(src->head_dim, view(src), view(dst), e, (hipStream_t)stream),
               "aspida_kv4_evict_dev");
+}
+
+extern "C" int aspida_tree_dev(const int* parent, int n_rows, int n_seq, const int* row_start, const int* kv_len,
+                               int* pos, unsigned* mask, int mask_words, void* stream) {
+  kq::Kv4Rows r;
+  if (mask && (mask_words < 1 || mask_words > kq::TREE_MAX_WORDS)) return -EINVAL;
+  if (const int rc = rows_of(n_rows, n_seq, row_start, kv_len, r)) return rc < 0 ? rc : 0;
+  if (!aligned(parent, 4) || (pos && !aligned(pos, 4)) || (mask && !aligned(mask, 4))) return -EINVAL;
+  return done(kq::launch_tree({parent, r.row_start, r.kv_len, n_rows, n_seq}, pos, mask, mask_words,
+                              (hipStream_t)stream),
+              "aspida_tree_dev");
+}
+
+extern "C" long long aspida_kv4_tree_attn_work_bytes(const aspida_kv4* cache, int n_heads, int n_rows, int n_seq,
+                                                     int max_rows) {
+  if (max_rows > kq::TREE_MAX_ROWS) return -EINVAL;
+  return aspida_kv4_attn_work_bytes(cache, n_heads, n_rows, n_seq, max_rows);
+}
+
+extern "C" int aspida_kv4_tree_attn_dev(const aspida_kv4* cache, int type, const void* q, long long q_stride,
+                                        int n_heads, int n_rows, int n_seq, const int* row_start, int max_rows,
+                                        const int* kv_len, const unsigned* mask, int mask_words, float scale,
+                                        int window, void* out, long long out_stride, float* lse, void* work,
+                                        void* stream) {
+  if (!valid_cache(cache) || !valid_heads(cache, n_heads) || max_rows < 1 || max_rows > kq::TREE_MAX_ROWS ||
+      mask_words < 1 || mask_words > kq::TREE_MAX_WORDS || window < 0 || !std::isfinite(scale))
+    return -EINVAL;
+  kq::Kv4Rows r;
+  if (const int rc = rows_of(n_rows, n_seq, row_start, kv_len, r)) return rc < 0 ? rc : 0;
+  if (!valid_rows(q, type, q_stride, n_heads, cache->head_dim) ||
+      !valid_rows(out, type, out_stride, n_heads, cache->head_dim) || !aligned(mask, 4) || (lse && !aligned(lse, 4)) ||
+      !aligned(work, 256))
+    return -EINVAL;
+  const int rows = longest(max_rows, n_rows);
+  // Column tiles of all kv heads are a dimension of the launch.
+  if (((long long)rows * (n_heads / cache->n_kv) + 15) / 16 * cache->n_kv > 65535) return -ENOTSUP;
+  kq::Kv4Attn a{q, q_stride, out, out_stride, lse, work, n_heads, rows, window, scale, mask, mask_words};
+  return done(kq::launch_kv4_attn(cache->head_dim, view(cache), type, r, a, (hipStream_t)stream),
+              "aspida_kv4_tree_attn_dev");
+}
+
+extern "C" int aspida_kv4_keep_dev(const aspida_kv4* cache, int n_rows, int n_seq, const int* row_start,
+                                   const int* kv_len, const int* path, const int* count, void* stream) {
+  if (!valid_cache(cache)) return -EINVAL;
+  kq::Kv4Rows r;
+  if (const int rc = rows_of(n_rows, n_seq, row_start, kv_len, r)) return rc < 0 ? rc : 0;
+  if (!aligned(path, 4) || !aligned(count, 4)) return -EINVAL;
+  return done(kq::launch_kv4_keep(cache->head_dim, view(cache), r, path, count, (hipStream_t)stream),
+              "aspida_kv4_keep_dev");
+}
+
+extern "C" long long aspida_tree_accept_work_bytes(int n_rows, int vocab) {
+  if (n_rows < 0 || n_rows > (1 << 22) || vocab < 1 || vocab > (1 << 30)) return -EINVAL;
+  return (long long)kq::tree_accept_work_bytes(n_rows > 0 ? n_rows : 1, vocab);
+}
+
+extern "C" int aspida_tree_accept_dev(int type, const void* logits, long long stride, int vocab, int n_rows, int n_seq,
+                                      const int* row_start, const int* kv_len, const int* parent, const int* token,
+                                      int* path, int* count, int* next, int* new_len, void* work, void* stream) {
+  if (!type_bytes(type) || vocab < 1 || vocab > (1 << 30) || stride < vocab || n_rows > (1 << 22)) return -EINVAL;
+  kq::Kv4Rows r;
+  if (const int rc = rows_of(n_rows, n_seq, row_start, kv_len, r)) return rc < 0 ? rc : 0;
+  if (!aligned(logits, (size_t)type_bytes(type)) || !aligned(parent, 4) || !aligned(token, 4) || !aligned(path, 4) ||
+      !aligned(count, 4) || !aligned(next, 4) || !aligned(new_len, 4) || !aligned(work, 8))
+    return -EINVAL;
+  kq::TreeAccept a{logits, stride, vocab, token, path, count, next, new_len, work};
+  return done(kq::launch_tree_accept(type, {parent, r.row_start, r.kv_len, n_rows, n_seq}, a, (hipStream_t)stream),
+              "aspida_tree_accept_dev");
 }

@@ -3,7 +3,9 @@
 // Row i of a sequence's n new rows sits at slot p = kv_len - n + i and sees
 // the slots j <= p (and j > p - window):
 //   o = sum_j softmax_j(scale q . k_j) v_j,   lse = log sum_j exp(scale q . k_j).
-// A row that sees nothing gets o = 0 and lse = -inf.
+// A row that sees nothing gets o = 0 and lse = -inf.  Rows that are a tree
+// (TREE) see the slots j < kv_len - n, and of the n rows those that their mask
+// names; with a window, so many of the former that it sees `window` in all.
 //
 // kv4_attn_split: the rows of a sequence times the query heads of a kv head
 // are columns, 16 to a tile.  A wave takes 32 tokens at a time:
@@ -51,11 +53,13 @@ constexpr float LN2 = 0.6931471805599453f;
 
 // Slots that a sequence's rows see together: [lo, hi), lo a multiple of 32.
 struct SeenRange { int lo, hi; };
+template <bool TREE>
 __device__ __forceinline__ SeenRange seen_range(const Kv4Span& s, int window, int max_slots) {
   const int first = s.len - (s.r1 - s.r0);  // the first row's slot
   SeenRange r;
   r.hi = s.r1 > s.r0 ? min(s.len, max_slots) : 0;
-  r.lo = min(kv4_lowest(first, kv4_reach(window)), r.hi) & ~31;
+  const int lowest = TREE ? (window > 0 ? max(0, max(first, 0) - window) : 0) : kv4_lowest(first, kv4_reach(window));
+  r.lo = min(lowest, r.hi) & ~31;
   return r;
 }
 
@@ -64,8 +68,9 @@ __device__ __forceinline__ SeenRange seen_range(const Kv4Span& s, int window, in
 // sequence besides: its rows, page ids and sums, about 8000 cycles where a
 // round takes 1800.
 constexpr int AXIS_EXTRA = 4;
+template <bool TREE>
 __device__ __forceinline__ int rounds_of(const Kv4Span& s, int window, int max_slots) {
-  const SeenRange r = seen_range(s, window, max_slots);
+  const SeenRange r = seen_range<TREE>(s, window, max_slots);
   return max(1, (r.hi - r.lo + ATTN_STEP - 1) / ATTN_STEP);
 }
 
@@ -86,21 +91,23 @@ __device__ __forceinline__ long long wave_scan64(long long v) {
 
 // own: the span of sequence `lane`, which the first 64 sequences' lengths come
 // from.
+template <bool TREE>
 __device__ __forceinline__ long long axis_total(const Kv4Rows& rows, const Kv4Span& own, int window, int max_slots) {
   const int lane = threadIdx.x & 63;
-  long long total = lane < rows.n_seq ? rounds_of(own, window, max_slots) + AXIS_EXTRA : 0;
-  for (int b = 64 + lane; b < rows.n_seq; b += 64) total += rounds_of(kv4_span(rows, b), window, max_slots) + AXIS_EXTRA;
+  long long total = lane < rows.n_seq ? rounds_of<TREE>(own, window, max_slots) + AXIS_EXTRA : 0;
+  for (int b = 64 + lane; b < rows.n_seq; b += 64) total += rounds_of<TREE>(kv4_span(rows, b), window, max_slots) + AXIS_EXTRA;
 #pragma unroll
   for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o, 64);
   return total;
 }
 
+template <bool TREE>
 __device__ __forceinline__ AxisPlace axis_place(const Kv4Rows& rows, const Kv4Span& own, int window, int max_slots,
                                                 int groups, int x) {
   const int lane = threadIdx.x & 63;
   AxisPlace p;
   if (rows.n_seq <= 64) {  // one lane each, and sums below 2^30
-    const int n = lane < rows.n_seq ? rounds_of(own, window, max_slots) + AXIS_EXTRA : 0;
+    const int n = lane < rows.n_seq ? rounds_of<TREE>(own, window, max_slots) + AXIS_EXTRA : 0;
     const int end = wave_scan_add(n);
     p.share = (__builtin_amdgcn_readlane(end, 63) + groups - 1) / groups;
     p.x0 = x * p.share;
@@ -110,12 +117,12 @@ __device__ __forceinline__ AxisPlace axis_place(const Kv4Rows& rows, const Kv4Sp
     p.start = __builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(n, l);
     return p;
   }
-  p.share = (axis_total(rows, own, window, max_slots) + groups - 1) / groups;
+  p.share = (axis_total<TREE>(rows, own, window, max_slots) + groups - 1) / groups;
   p.x0 = x * p.share;
   long long before = 0;
   for (int b0 = 0; b0 < rows.n_seq; b0 += 64) {
     const int b = b0 + lane;
-    const int n = b < rows.n_seq ? rounds_of(b0 ? kv4_span(rows, b) : own, window, max_slots) + AXIS_EXTRA : 0;
+    const int n = b < rows.n_seq ? rounds_of<TREE>(b0 ? kv4_span(rows, b) : own, window, max_slots) + AXIS_EXTRA : 0;
     const long long end = before + wave_scan64(n);
     const uint64_t over = __ballot(end > p.x0);
     if (over) {
@@ -169,7 +176,43 @@ __device__ void fill_excess(const SplitArgs& s, const Kv4Span& sp, int hk, int d
   }
 }
 
-template <int D, class T>
+// What a column of a tree sees: the slots [lo, base) and the rows [r0, r1)
+// that its mask names.
+struct TreeSeen {
+  const uint32_t* mask;
+  int lo, r0, r1;
+  __device__ __forceinline__ uint32_t word(int w) const {
+    uint32_t v = 32 * w < r1 && 32 * w + 32 > r0 ? mask[w] : 0u;
+    if (32 * w + 32 > r1) v &= r1 - 32 * w > 0 ? ~0u >> (32 * w + 32 - r1) : 0u;
+    if (32 * w < r0) v &= r0 - 32 * w < 32 ? ~0u << (r0 - 32 * w) : 0u;
+    return v;
+  }
+  // Bits of the rows j .. j + 31 (j may be below 0).
+  __device__ __forceinline__ uint32_t rows(int j) const {
+    const int w = j >> 5;
+    return __builtin_amdgcn_alignbit(word(w + 1), word(w), (uint32_t)(j & 31));
+  }
+  __device__ __forceinline__ TreeSeen() : mask(nullptr), lo(0), r0(0), r1(0) {}
+  // n rows at slots from base on, of which those at slots below 0 do not count.
+  __device__ __forceinline__ TreeSeen(const Kv4Attn& a, int row0, int row, int n, int base, bool valid) {
+    r0 = max(0, -base);
+    r1 = valid && base + row >= 0 ? min(n, 32 * a.mask_words) : 0;
+    mask = a.mask + (size_t)(row0 + (r1 > 0 ? row : 0)) * a.mask_words;
+    int shown = 0;
+    if (a.window > 0)
+      for (int w = 0; 32 * w < r1; ++w) shown += __popc(word(w));
+    lo = r1 <= 0 ? max(base, 0) : a.window > 0 ? max(0, max(base, 0) - max(a.window - shown, 0)) : 0;
+  }
+  // Whether it sees a slot from max_slots on.
+  __device__ __forceinline__ bool past(int base, int max_slots) const {
+    if (lo < base && base > max_slots) return true;
+    bool any = false;
+    for (int j = max(0, max_slots - base); j < r1; j += 32) any |= rows(j) != 0;
+    return any;
+  }
+};
+
+template <int D, class T, bool TREE>
 __global__ __launch_bounds__(64 * ATTN_WAVES, D == 64 ? 3 : D == 128 ? 2 : 1) void kv4_attn_split(SplitArgs s) {
   using L = Kv4L<D>;
   constexpr bool TWO = sizeof(T) == 4;
@@ -183,7 +226,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, D == 64 ? 3 : D == 128 ? 2 : 1) vo
   const int mine = threadIdx.x & 63;
   Kv4Span own = {0, 0, 0};
   if (mine < s.rows.n_seq) own = kv4_span(s.rows, mine);
-  AxisPlace place = axis_place(s.rows, own, s.a.window, max_slots, s.groups, blockIdx.x);
+  AxisPlace place = axis_place<TREE>(s.rows, own, s.a.window, max_slots, s.groups, blockIdx.x);
   const long long x1 = place.x0 + place.share;
   for (int b = place.seq; b < s.rows.n_seq && place.start < x1; ++b) {
     // (Opaque, so that what follows from it is not kept in registers from one
@@ -199,8 +242,8 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, D == 64 ? 3 : D == 128 ? 2 : 1) vo
     } else {
       sp = kv4_span(s.rows, b);
     }
-    const SeenRange seen = seen_range(sp, s.a.window, max_slots);
-    const int length = rounds_of(sp, s.a.window, max_slots);
+    const SeenRange seen = seen_range<TREE>(sp, s.a.window, max_slots);
+    const int length = rounds_of<TREE>(sp, s.a.window, max_slots);
     // Its rounds [u0, u1) are in this share.
     const long long at = place.start + AXIS_EXTRA;
     place.start = at + length;
@@ -220,16 +263,32 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, D == 64 ? 3 : D == 128 ? 2 : 1) vo
     // The share's slots, and those of them that every column sees.
     const int t0 = seen.lo + u0 * ATTN_STEP, t1 = (int)min((long long)seen.hi, seen.lo + (long long)u1 * ATTN_STEP);
     const int row_last = (tile * 16 + ncol - 1) / s.group, row_first = tile * 16 / s.group;
-    const int all_hi = sp.len - n + row_first + 1;                                       // below: seen by every column
-    const int all_lo = kv4_lowest(sp.len - n + row_last, reach);
-    const int any_hi = min(t1, sp.len - n + row_last + 1);
-    const int any_lo = kv4_lowest(sp.len - n + row_first, reach);
+    int all_hi = sp.len - n + row_first + 1;  // below: seen by every column
+    int all_lo = kv4_lowest(sp.len - n + row_last, reach);
+    int any_hi = min(t1, sp.len - n + row_last + 1);
+    int any_lo = kv4_lowest(sp.len - n + row_first, reach);
+    const int base = sp.len - n;
+    const TreeSeen tree = TREE ? TreeSeen(s.a, sp.r0, row, n, base, valid) : TreeSeen();
+    if constexpr (TREE) {
+      any_lo = valid ? tree.lo : base;
+      all_lo = valid ? tree.lo : 0;
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) {
+        any_lo = min(any_lo, __shfl_xor(any_lo, o, 64));
+        all_lo = max(all_lo, __shfl_xor(all_lo, o, 64));
+      }
+      any_lo = __builtin_amdgcn_readfirstlane(any_lo);
+      all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+      all_hi = base;
+      any_hi = t1;
+    }
 
     kvf4 o[NT], om = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NT; ++i) o[i] = om;
     // A row past the table sees its own slot there: NaN.
-    float ref = REF0, l = chi > max_slots && u0 == 0 && wave == 0 ? __builtin_nanf("") : 0.f;
+    const bool past = TREE ? u0 == 0 && wave == 0 && tree.past(base, max_slots) : chi > max_slots && u0 == 0 && wave == 0;
+    float ref = REF0, l = past ? __builtin_nanf("") : 0.f;
 
     // Two sets of registers: one is multiplied while the other arrives.  The
     // loads are the same every time (past the end they read any page again), so
@@ -262,12 +321,22 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, D == 64 ? 3 : D == 128 ? 2 : 1) vo
         // Slots that this column does not see get no weight; the steps and
         // minima of slots that no column sees may be anything and become 0.
         uint32_t keep = 0;
+        // A tree: bit i of sees is slot at + i for this column, of some for any of them.
+        uint32_t sees = 0, some = 0;
+        if constexpr (TREE) {
+          if (at + 32 > base) sees = tree.rows(at - base);
+          const int lo = tree.lo - at, hi = base - at;
+          if (hi > 0 && lo < 32 && lo < hi) sees |= (hi < 32 ? ~(~0u << hi) : ~0u) & (lo > 0 ? ~0u << lo : ~0u);
+          some = sees;
+#pragma unroll
+          for (int o = 1; o < 16; o <<= 1) some |= (uint32_t)__shfl_xor((int)some, o, 64);
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int slot = at + 16 * (j >> 2) + 4 * rg + (j & 3);
-          const bool see = slot >= clo && slot < chi;
+          const int in = 16 * (j >> 2) + 4 * rg + (j & 3), slot = at + in;
+          const bool see = TREE ? sees >> in & 1 : slot >= clo && slot < chi;
           x[j] = see ? (y.there ? x[j] * unit : __builtin_nanf("")) : -INFINITY;
-          if (y.there && slot < any_hi && slot >= any_lo) keep |= 1u << j;
+          if (y.there && (TREE ? some >> in & 1 : slot < any_hi && slot >= any_lo)) keep |= 1u << j;
         }
         y.v.drop(keep);
         u = 1.f;
@@ -394,7 +463,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, D == 64 ? 3 : D == 128 ? 2 : 1) vo
 // Joins the parts of a sequence: a workgroup per (column of a kv head's
 // tile, sequence).  Each of its waves takes every fourth part, 64 lanes over
 // the dims; LDS adds the four up.
-template <int D, class T>
+template <int D, class T, bool TREE>
 __global__ __launch_bounds__(256) void kv4_attn_join(SplitArgs s) {
   constexpr int E = D / 64;
   __shared__ float so[4][D], sl[4];
@@ -408,21 +477,21 @@ __global__ __launch_bounds__(256) void kv4_attn_join(SplitArgs s) {
   if (lane < s.rows.n_seq) own = kv4_span(s.rows, lane);
   long long total, start;  // the axis, and where this sequence begins on it
   if (s.rows.n_seq <= 64) {
-    const int n = lane < s.rows.n_seq ? rounds_of(own, s.a.window, max_slots) + AXIS_EXTRA : 0;
+    const int n = lane < s.rows.n_seq ? rounds_of<TREE>(own, s.a.window, max_slots) + AXIS_EXTRA : 0;
     const int upto = wave_scan_add(n);
     total = __builtin_amdgcn_readlane(upto, 63);
     start = __builtin_amdgcn_readlane(upto, b) - __builtin_amdgcn_readlane(n, b);
   } else {
-    total = axis_total(s.rows, own, s.a.window, max_slots);
-    start = lane < b ? rounds_of(own, s.a.window, max_slots) + AXIS_EXTRA : 0;
+    total = axis_total<TREE>(s.rows, own, s.a.window, max_slots);
+    start = lane < b ? rounds_of<TREE>(own, s.a.window, max_slots) + AXIS_EXTRA : 0;
     for (int i = 64 + lane; i < b; i += 64)
-      start += rounds_of(kv4_span(s.rows, i), s.a.window, max_slots) + AXIS_EXTRA;
+      start += rounds_of<TREE>(kv4_span(s.rows, i), s.a.window, max_slots) + AXIS_EXTRA;
 #pragma unroll
     for (int o = 32; o; o >>= 1) start += __shfl_xor(start, o, 64);
   }
   const long long share = (total + s.groups - 1) / s.groups;
   start += AXIS_EXTRA;
-  const long long first = start / share, last = (start + rounds_of(sp, s.a.window, max_slots) - 1) / share;
+  const long long first = start / share, last = (start + rounds_of<TREE>(sp, s.a.window, max_slots) - 1) / share;
   const int count = (int)(last - first) + 1;
   if (count == 1) return;
   // Its parts: number 2 first + 1, then 2 x of the workgroups behind.
@@ -471,29 +540,35 @@ size_t kv4_attn_work_bytes(int head_dim) {
                            : 2 * ATTN_GROUPS<256> * sizeof(AttnPart<256>);
 }
 
-template <int D, class T>
+template <int D, class T, bool TREE>
 static void attn_go(SplitArgs s, hipStream_t st) {
   const int per_seq = s.c.n_kv * s.tiles;
   s.groups = attn_groups<D>(per_seq);
-  hipLaunchKernelGGL((kv4_attn_split<D, T>), dim3(s.groups, per_seq), dim3(64 * ATTN_WAVES), 0, st, s);
+  hipLaunchKernelGGL((kv4_attn_split<D, T, TREE>), dim3(s.groups, per_seq), dim3(64 * ATTN_WAVES), 0, st, s);
   const int cols = (int)std::min<long long>(16, (long long)s.a.max_rows * s.group);
-  hipLaunchKernelGGL((kv4_attn_join<D, T>), dim3(cols, per_seq, s.rows.n_seq), dim3(256), 0, st, s);
+  hipLaunchKernelGGL((kv4_attn_join<D, T, TREE>), dim3(cols, per_seq, s.rows.n_seq), dim3(256), 0, st, s);
 }
 
-template <class T>
+template <class T, bool TREE>
 static void attn_typed(int head_dim, const SplitArgs& s, hipStream_t st) {
-  if (head_dim == 64) attn_go<64, T>(s, st);
-  else if (head_dim == 128) attn_go<128, T>(s, st);
-  else attn_go<256, T>(s, st);
+  if (head_dim == 64) attn_go<64, T, TREE>(s, st);
+  else if (head_dim == 128) attn_go<128, T, TREE>(s, st);
+  else attn_go<256, T, TREE>(s, st);
 }
 
 hipError_t launch_kv4_attn(int head_dim, const Kv4View& c, int type, const Kv4Rows& rows, const Kv4Attn& a,
                            hipStream_t st) {
-  if (kv4_prefill_takes(c, rows, a)) return launch_kv4_prefill(head_dim, c, type, rows, a, st);
+  if (!a.mask && kv4_prefill_takes(c, rows, a)) return launch_kv4_prefill(head_dim, c, type, rows, a, st);
   SplitArgs s{c, rows, a, a.n_heads / c.n_kv, attn_tiles(a.n_heads / c.n_kv, a.max_rows), 0};
-  if (type == ACT_F32) attn_typed<float>(head_dim, s, st);
-  else if (type == ACT_F16) attn_typed<_Float16>(head_dim, s, st);
-  else attn_typed<bf16_t>(head_dim, s, st);
+  if (a.mask) {
+    if (type == ACT_F32) attn_typed<float, true>(head_dim, s, st);
+    else if (type == ACT_F16) attn_typed<_Float16, true>(head_dim, s, st);
+    else attn_typed<bf16_t, true>(head_dim, s, st);
+  } else {
+    if (type == ACT_F32) attn_typed<float, false>(head_dim, s, st);
+    else if (type == ACT_F16) attn_typed<_Float16, false>(head_dim, s, st);
+    else attn_typed<bf16_t, false>(head_dim, s, st);
+  }
   return hipGetLastError();
 }
 

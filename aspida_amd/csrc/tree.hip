@@ -1,0 +1,160 @@
+// tree.hip -- trees of drafted tokens: masks and positions from parents, and
+// the greedy choice along a tree (contracts: include/aspidagpu.h).
+//
+// tree_accept: says(r) = the largest logit of row r, the lowest index among
+// equals (NaN never is one).  From row 0 on, the next row is the first child
+// whose token is what its parent says; where there is none, that is the next
+// token.  tree_says finds each row's largest in pieces (memory bound: all
+// logits are read once), tree_walk joins the pieces of a sequence's rows and
+// walks in LDS.
+#include <algorithm>
+
+#include "kq_common.h"
+#include "kv4.h"
+#include "tree.h"
+
+namespace kq {
+
+// A parent that is not an earlier row counts as none.
+__device__ __forceinline__ int tree_parent(const int* parent, int i) {
+  const int p = parent[i];
+  return p >= 0 && p < i ? p : -1;
+}
+
+// A workgroup per sequence: parents in LDS, then a thread for each word of
+// each row's mask climbs from the row until it is below the word's bits.
+__global__ __launch_bounds__(256) void tree_masks(TreeRows t, int* pos, uint32_t* mask, int words) {
+  __shared__ int16_t up[TREE_MAX_ROWS];
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const Kv4Span sp = kv4_span({t.row_start, t.kv_len, t.n_rows, t.n_seq}, b);
+  const int n = sp.r1 - sp.r0, m = min(n, TREE_MAX_ROWS);
+  for (int i = tid; i < m; i += 256) up[i] = (int16_t)tree_parent(t.parent + sp.r0, i);
+  __syncthreads();
+  if (mask)
+    for (long long x = tid; x < (long long)n * words; x += 256) {
+      const int i = (int)(x / words), w = (int)(x % words);
+      uint32_t bits = 0;
+      for (int j = i < m ? i : -1; j >= 32 * w; j = up[j])
+        if (j < 32 * w + 32) bits |= 1u << (j & 31);
+      mask[(size_t)sp.r0 * words + x] = bits;
+    }
+  if (pos)
+    for (int i = tid; i < n; i += 256) {
+      int depth = 0;
+      if (i < m)
+        for (int j = up[i]; j >= 0; j = up[j]) ++depth;
+      pos[sp.r0 + i] = sp.len - n + depth;
+    }
+}
+
+hipError_t launch_tree(const TreeRows& t, int* pos, uint32_t* mask, int words, hipStream_t s) {
+  hipLaunchKernelGGL(tree_masks, dim3(t.n_seq), dim3(256), 0, s, t, pos, mask, words);
+  return hipGetLastError();
+}
+
+struct Said { float v; int i; };  // a piece's largest logit and its index; INT_MAX: none
+
+__device__ __forceinline__ void say(Said& s, float v, int i) {
+  if (v > s.v || (v == s.v && i < s.i)) s = {v, i};
+}
+
+// 256 threads take elements [piece, piece + 1) * len of a row, eight
+// consecutive ones each in turn.
+template <class T>
+__global__ __launch_bounds__(256) void tree_says(const T* logits, long long stride, int vocab, int pieces, int len,
+                                                 Said* out) {
+  __shared__ Said part[4];
+  const int row = blockIdx.x / pieces, piece = blockIdx.x % pieces, tid = threadIdx.x;
+  const T* const x = logits + (long long)row * stride;
+  const int i0 = piece * len, i1 = (int)min((long long)vocab, (long long)i0 + len);
+  Said s = {-INFINITY, 0x7FFFFFFF};
+#pragma unroll 4
+  for (int i = i0 + 8 * tid; i + 8 <= i1; i += 8 * 256) {
+    struct { T t[8]; } r;
+    __builtin_memcpy(&r, x + i, sizeof(r));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) say(s, (float)r.t[j], i + j);
+  }
+  const int rest = i0 + (i1 - i0) / 8 * 8 + tid;
+  if (rest < i1) say(s, (float)x[rest], rest);
+  wave_argmax(s.v, s.i);
+  if ((tid & 63) == 0) part[tid >> 6] = s;
+  __syncthreads();
+  if (tid) return;
+  for (int w = 1; w < 4; ++w) say(s, part[w].v, part[w].i);
+  out[(size_t)row * pieces + piece] = s;
+}
+
+// A workgroup per sequence.
+__global__ __launch_bounds__(256) void tree_walk(TreeRows t, TreeAccept a, int pieces, int cap) {
+  extern __shared__ int lds[];  // says, token, parent of up to cap rows
+  __shared__ int found;
+  int *const says = lds, *const token = lds + cap, *const up = lds + 2 * cap;
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const Kv4Span sp = kv4_span({t.row_start, t.kv_len, t.n_rows, t.n_seq}, b);
+  const int n = sp.r1 - sp.r0, m = min(n, cap);
+  const Said* const in = (const Said*)a.work + (size_t)sp.r0 * pieces;
+  for (int i = tid; i < m; i += 256) {
+    Said s = {-INFINITY, 0x7FFFFFFF};
+    for (int p = 0; p < pieces; ++p) {
+      const Said u = in[(size_t)i * pieces + p];
+      say(s, u.v, u.i);
+    }
+    says[i] = s.i == 0x7FFFFFFF ? -1 : s.i;
+    token[i] = a.token[sp.r0 + i];
+    up[i] = tree_parent(t.parent + sp.r0, i);
+  }
+  int count = 0, said = -1;
+  for (int at = 0; at < m; ++count) {
+    if (tid == 0) {
+      found = m;
+      a.path[sp.r0 + count] = at;
+    }
+    __syncthreads();
+    said = says[at];
+    for (int i = at + 1 + tid; i < m; i += 256)
+      if (up[i] == at && token[i] == said && said >= 0) {
+        atomicMin(&found, i);
+        break;
+      }
+    __syncthreads();
+    at = found;
+    __syncthreads();
+  }
+  for (int i = count + tid; i < n; i += 256) a.path[sp.r0 + i] = -1;
+  if (tid == 0) {
+    a.count[b] = count;
+    a.next[b] = said;
+    a.new_len[b] = max(sp.len - n + count, 0);
+  }
+}
+
+// Pieces of a row: about 2048 workgroups in all, of at least 4096 elements.
+static int says_pieces(int n_rows, int vocab) {
+  return (int)std::max<long long>(1, std::min<long long>((2048 + n_rows - 1) / n_rows, (vocab + 4095) / 4096));
+}
+
+size_t tree_accept_work_bytes(int n_rows, int vocab) {
+  return ((size_t)n_rows * says_pieces(n_rows, vocab) * sizeof(Said) + 255) / 256 * 256;
+}
+
+template <class T>
+static void says_go(const TreeRows& t, const TreeAccept& a, int pieces, int len, hipStream_t s) {
+  hipLaunchKernelGGL(tree_says<T>, dim3((unsigned)(t.n_rows * pieces)), dim3(256), 0, s, (const T*)a.logits, a.stride,
+                     a.vocab, pieces, len, (Said*)a.work);
+}
+
+hipError_t launch_tree_accept(int type, const TreeRows& t, const TreeAccept& a, hipStream_t s) {
+  const int pieces = says_pieces(t.n_rows, a.vocab);
+  const int len = (a.vocab / 8 + pieces) / pieces * 8;  // whole runs of eight; pieces * len >= vocab
+  if (type == ACT_F32) says_go<float>(t, a, pieces, len, s);
+  else if (type == ACT_F16) says_go<_Float16>(t, a, pieces, len, s);
+  else says_go<bf16_t>(t, a, pieces, len, s);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const int cap = std::min(t.n_rows, TREE_MAX_ROWS);
+  hipLaunchKernelGGL(tree_walk, dim3(t.n_seq), dim3(256), 3 * sizeof(int) * cap, s, t, a, pieces, cap);
+  return hipGetLastError();
+}
+
+}  // namespace kq

@@ -353,6 +353,96 @@ int aspida_kv4_evict_dev(const aspida_kv4 *src, int n_seq, const int *kv_len, co
                          int keep, int first, int recent, const aspida_kv4 *dst, int *new_len, int *idx,
                          float *acc_out, void *stream);
 
+/* ---- trees of drafted tokens over the cache ------------------------------------
+ * A step of speculative decoding: a sequence's rows are a tree, row 0 the last
+ * token that is sure and every other row a drafted token behind its parent, an
+ * earlier row of the sequence (parent: row number within the sequence; a value
+ * that names no earlier row, such as -1, names none).  Rows and lengths are
+ * those of the calls above, so that kv4_append writes a tree's keys and values
+ * at slots base .. kv_len - 1, base = kv_len - rows.  At most 4096 rows a
+ * sequence.  All calls may be captured, and allocate nothing. */
+
+/* From parents [n_rows]: pos[row] = base + its depth (what a rotation takes),
+ * mask[row][mask_words]: bit j % 32 of word j / 32 is set for the row's
+ * ancestors and itself (mask_words 1 to 128: words past it are not written).
+ * Either may be NULL. */
+int aspida_tree_dev(const int *parent, int n_rows, int n_seq, const int *row_start, const int *kv_len, int *pos,
+                    unsigned *mask, int mask_words, void *stream);
+
+/* aspida_kv4_attn_dev for such rows: a row sees the slots before base, and of
+ * its sequence's rows those that its mask names (any of them, itself or not;
+ * rows past 32 * mask_words are not seen).  With window > 0 it sees `window`
+ * slots in all: the rows that its mask names, and as many of the last slots
+ * before base as remain.  A row that sees nothing gets 0, and lse -inf; rows
+ * at slots below 0 see nothing and are not seen.  max_rows (up to 4096) as
+ * there.  -ENOTSUP for more than 65535 tiles of 16 columns (max_rows * heads of
+ * a kv head) in all kv heads. */
+long long aspida_kv4_tree_attn_work_bytes(const aspida_kv4 *cache, int n_heads, int n_rows, int n_seq, int max_rows);
+int aspida_kv4_tree_attn_dev(const aspida_kv4 *cache, int type, const void *q, long long q_stride, int n_heads,
+                             int n_rows, int n_seq, const int *row_start, int max_rows, const int *kv_len,
+                             const unsigned *mask, int mask_words, float scale, int window, void *out,
+                             long long out_stride, float *lse, void *work, void *stream);
+
+/* The greedy choice along each tree.  A row says the token of its largest
+ * logit (logits [n_rows][vocab] of `type`, rows `stride` elements apart; the
+ * lowest index among equals; NaN never is the largest).  Starting at row 0,
+ * the next row is the first child of the last one whose token[n_rows] is what
+ * the last one says; where there is none, that is the next token.  path: the
+ * accepted rows' numbers within the sequence, from path[row_start[b]] on (row 0
+ * among them; -1 behind them); count[b] how many; next[b] what the last one
+ * says (-1 where all its logits are NaN, or the sequence has no rows);
+ * new_len[b] = base + count[b] (new_len may be kv_len).  path may not be
+ * parent or token.  work: aspida_tree_accept_work_bytes, 8-byte aligned. */
+long long aspida_tree_accept_work_bytes(int n_rows, int vocab);
+int aspida_tree_accept_dev(int type, const void *logits, long long stride, int vocab, int n_rows, int n_seq,
+                           const int *row_start, const int *kv_len, const int *parent, const int *token, int *path,
+                           int *count, int *next, int *new_len, void *work, void *stream);
+
+/* The accepted rows moved together: slot base + i takes what slot base +
+ * path[row_start[b] + i] held, for i < count[b]; kv_len is the length with the
+ * whole tree (the one the rows were appended with).  Entries must ascend and
+ * name rows of the sequence: the first that does not ends the path.  Codes are
+ * moved, not rounded again; slots behind the kept ones stay as they were. */
+int aspida_kv4_keep_dev(const aspida_kv4 *cache, int n_rows, int n_seq, const int *row_start, const int *kv_len,
+                        const int *path, const int *count, void *stream);
+
+/* ---- products with 8-bit integer weights ----------------------------------------
+ * Weights as int8 codes with an f32 scale per row (output channel), activations
+ * quantised by the call with a scale per token:
+ *   s_x = f32(max |x| / 127), c_x = x / s_x rounded to nearest (ties to even),
+ *   y[t][o] = s_x[t] s_w[o] sum_k c_x[t][k] c_w[o][k],
+ * the sum exact, the rest in f32 and rounded to the type once.  A token whose
+ * largest magnitude is below 2^-100 counts as zeros; a token (or a weight row
+ * in aspida_w8_convert_dev) with a value that is not finite comes out as NaN
+ * in all its results.  Activation types as above: 0 f32, 1 f16, 2 bf16; any
+ * in_dim up to 131072 and out_dim up to 2^22, operands aligned to their type,
+ * rows x_stride >= in_dim and y_stride >= out_dim elements apart.  No
+ * counterpart in the reference ABI.  For inference: there is no gradient. */
+
+/* Bytes of packed weights (or -EINVAL); they are 16-byte aligned. */
+long long aspida_w8_bytes(int in_dim, int out_dim);
+/* Packed once per weight: from int8 codes [out_dim] rows `stride` apart (any
+ * values, -128 to 127) and scale[out_dim] (any values). */
+int aspida_w8_pack_dev(const signed char *codes, long long stride, const float *scale, int in_dim, int out_dim,
+                       void *packed, void *stream);
+/* Packed from a matrix of a quantised kind (0..5, in_dim a multiple of 256) or
+ * of f32 (-1): each row with the scale f32(max |w| / 127) and nearest codes. */
+int aspida_w8_convert_dev(int kind, const void *w, int in_dim, int out_dim, void *packed, void *stream);
+/* The values that packed weights stand for, w f32 [out_dim][in_dim]. */
+int aspida_w8_unpack_dev(const void *packed, int in_dim, int out_dim, float *w, void *stream);
+
+/* y[n_rows][out_dim] of x[n_rows][in_dim].  work: aspida_w8_work_bytes, 256-byte
+ * aligned; launches that share it must be ordered.  y must not overlap x.
+ * Nothing is allocated; the calls may be captured. */
+long long aspida_w8_work_bytes(int n_rows, int in_dim);
+int aspida_w8_matmul_dev(const void *packed, int in_dim, int out_dim, int type, const void *x, long long x_stride,
+                         int n_rows, void *y, long long y_stride, void *work, void *stream);
+/* The gated feed-forward block in one call: y = act(gate x) * (up x), both
+ * weights [out_dim][in_dim] packed, act 0: silu(g) = g / (1 + e^-g), 1: gelu in
+ * its tanh form.  Neither projection is rounded to the type or stored. */
+int aspida_w8_gated_dev(const void *gate, const void *up, int in_dim, int out_dim, int act, int type, const void *x,
+                        long long x_stride, int n_rows, void *y, long long y_stride, void *work, void *stream);
+
 /* Resident decode chain: an ordered list of packed matvecs (steps) run by ONE
  * persistent launch, with no launch boundary between them -- e.g. every
  * weight matrix of a decoder pass.  A step whose x lies inside an earlier
