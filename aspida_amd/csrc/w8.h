@@ -57,9 +57,14 @@ hipError_t launch_w8(int type, const W8Args& a, hipStream_t s);
 
 #ifdef __HIPCC__
 typedef int w8i4 __attribute__((ext_vector_type(4)));
+typedef int w8i16 __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ w8i4 w8_mfma(w8i4 a, w8i4 b, w8i4 c) {
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ w8i16 w8_mfma32(w8i4 a, w8i4 b, w8i16 c) {
+  return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
 }
 
 // A row's scale from its largest magnitude (NaN where a value is not finite:
@@ -95,49 +100,85 @@ struct W8Unit {
   int e;
   __device__ __forceinline__ explicit W8Unit(float s) : m(__builtin_amdgcn_frexp_mantf(s)), e(__builtin_amdgcn_frexp_expf(s)) {}
 };
-__device__ __forceinline__ float w8_value(int sum, const W8Unit& a, const W8Unit& b) {
-  return __builtin_ldexpf((float)sum * a.m * b.m, a.e + b.e);
+__device__ __forceinline__ float w8_value(int sum, float m, int e, const W8Unit& b) {
+  return __builtin_ldexpf((float)sum * m * b.m, e + b.e);
 }
 
 // act(g) u, act(g) = g / (1 + e^-t): t = g is silu, t = 2 sqrt(2 / pi) (g +
 // 0.044715 g^3) gelu in its tanh form.  For t < 0 it is g e^t / (1 + e^t), e^t
-// multiplied in as two roots: the result alone, and nothing before it, leaves
-// f32's range.
+// multiplied in as two roots, so that nothing but the result leaves f32's
+// range (down to t = -174, where the roots do).  exp2 and the reciprocal of a
+// number in [1, 2] are the instructions', good to an ulp: a prompt's 30 million
+// results would otherwise spend as long here as an eighth of their products.
 __device__ __forceinline__ float w8_gate(float g, float u, int act) {
   const float t = act == 0 ? g : 1.5957691216057308f * __builtin_fmaf(0.044715f * g * g, g, g);
-  const float h = expf(-0.5f * __builtin_fabsf(t)), den = __builtin_fmaf(h, h, 1.f);
-  return t < 0.f ? g * h * u * h / den : g / den * u;
+  const float h = __builtin_amdgcn_exp2f(-0.72134752044448170368f * __builtin_fabsf(t));
+  const float p = t < 0.f ? h : 1.f;
+  return g * p * u * p * __builtin_amdgcn_rcpf(__builtin_fmaf(h, h, 1.f));
 }
 
-// 16 consecutive activations from x + k as f32; past in_dim zeros.
-template <class T>
-__device__ __forceinline__ void w8_load16(const T* x, int k, int in_dim, float (&v)[16]) {
-  if (k + 16 <= in_dim) {
-    struct { T t[16]; } r;
-    __builtin_memcpy(&r, x + k, sizeof(r));
+// Runs of 16 consecutive activations.  w8_run: a whole one, at any alignment
+// of the type; w8_rest: the one that in_dim ends in, zeros behind it.
+template <class T> struct W8Run {
+  T t[16];
+  __device__ __forceinline__ void values(float (&v)[16]) const {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = (float)r.t[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = k + i < in_dim ? (float)x[k + i] : 0.f;
+    for (int i = 0; i < 16; ++i) v[i] = (float)t[i];
   }
+};
+template <class T> __device__ __forceinline__ W8Run<T> w8_run(const T* x) {
+  W8Run<T> r;
+  __builtin_memcpy(&r, x, sizeof(r));
+  return r;
+}
+template <class T> __device__ __forceinline__ W8Run<T> w8_rest(const T* x, int n) {
+  W8Run<T> r;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) r.t[i] = i < n ? x[i] : (T)0.f;
+  return r;
 }
 // The larger magnitude; infinite where one is not finite.
 __device__ __forceinline__ float w8_top(float top, float v) {
   const float a = __builtin_fabsf(v);
   return a <= 3.402823466e38f ? __builtin_fmaxf(top, a) : __builtin_inff();
 }
-__device__ __forceinline__ float w8_top16(const float (&v)[16], float top) {
+// Magnitudes as bits, which order as the numbers do; NaN above infinity.
+template <class T> __device__ __forceinline__ uint32_t w8_top16(const W8Run<T>& r, uint32_t top) {
+  float v[16];
+  r.values(v);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) top = w8_top(top, v[i]);
+  for (int i = 0; i < 16; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu);
   return top;
 }
-__device__ __forceinline__ uint4 w8_codes16(const float (&v)[16], const W8Scale& s) {
+// 16 codes of a wave's lanes at a time.  x inv + 1.5 2^23, rounded once, has
+// the code in its lowest byte; x inv is off by at most 127 2^-24, so only
+// where one comes within 2^-16 of a half are the lane's codes settled one by
+// one (three steps of 1024 values in a hundred).  That is 5 instructions a
+// value in place of about 20, which were most of the time of long rows.
+template <class T> __device__ __forceinline__ uint4 w8_codes16(const W8Run<T>& run, const W8Scale& s) {
+  constexpr float M = 12582912.f;
+  float v[16], r[16], far = 0.f;
+  run.values(v);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    r[i] = __builtin_fmaf(v[i], s.inv, M);
+    far = __builtin_fmaxf(far, __builtin_fabsf(__builtin_fmaf(v[i], s.inv, M - r[i])));
+  }
   uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = w8_four(s.code(v[4 * i]), s.code(v[4 * i + 1]), s.code(v[4 * i + 2]), s.code(v[4 * i + 3]));
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  for (int i = 0; i < 4; ++i) {
+    auto bits = [&](int j) { return __builtin_bit_cast(uint32_t, r[4 * i + j]); };
+    // Bytes of (a, b): 0..3 are b's, 4..7 a's.
+    const uint32_t lo = __builtin_amdgcn_perm(bits(1), bits(0), 0x0C0C0400u), hi = __builtin_amdgcn_perm(bits(3), bits(2), 0x04000C0Cu);
+    w[i] = lo | hi;
+  }
+  if (__ballot(far > 0.5f - 0x1p-16f)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = w8_four(s.code(v[4 * i]), s.code(v[4 * i + 1]), s.code(v[4 * i + 2]), s.code(v[4 * i + 3]));
+  }
+  return s.inv == 0.f ? make_uint4(0, 0, 0, 0) : make_uint4(w[0], w[1], w[2], w[3]);
 }
+
 // Where codes k .. k + 15 (k a multiple of 16) of a row stand.
 __device__ __forceinline__ size_t w8_place(int row, int k, int blocks) {
   return ((size_t)(row >> 4) * blocks + (k >> 6)) * W8_TILE + ((k >> 4 & 3) * 16 + (row & 15)) * 16;
@@ -146,18 +187,20 @@ __device__ __forceinline__ float* w8_scales(const uint8_t* packed, int in_dim, i
   return reinterpret_cast<float*>(const_cast<uint8_t*>(packed) + w8_code_bytes(in_dim, rows));
 }
 
-// Largest value over a workgroup of NW waves, in every thread.
-template <int NW>
-__device__ __forceinline__ float w8_group_max(float v, float* lds) {
+// Largest value over a wave, and over a workgroup of NW waves, in every thread.
+template <class V> __device__ __forceinline__ V w8_wave_max(V v) {
 #pragma unroll
-  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  if constexpr (NW > 1) {
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = lds[0];
+  for (int o = 32; o; o >>= 1) v = max(v, (V)__shfl_xor(v, o, 64));
+  return v;
+}
+template <int NW, class V>
+__device__ __forceinline__ V w8_group_max(V v, V* lds) {
+  v = w8_wave_max(v);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = lds[0];
 #pragma unroll
-    for (int i = 1; i < NW; ++i) v = fmaxf(v, lds[i]);
-  }
+  for (int i = 1; i < NW; ++i) v = max(v, lds[i]);
   return v;
 }
 #endif
