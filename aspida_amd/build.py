@@ -32,13 +32,14 @@ CFLAGS = [
 # from the 64-row column loops (Q2_K / Q3_K / Q5_K launches of 28672x4096 and
 # up 2-7% faster, the 8B decode +0.2%); the small-batch sources measured equal
 # or slower with it (Q4_K 4096^2 at 64 vectors +12%), so only this file.
-# kv4_attn.hip, kv4_weigh.hip, kv4_prefill.hip, w8_gemm.hip, w8_rows.hip: without it the sums sit in
+# kv4_attn.hip, kv4_weigh.hip, kv4_prefill.hip, kv4_tree.hip, w8_gemm.hip, w8_rows.hip: without it the sums sit in
 # AGPRs, and every product with a vector instruction moves them (decode
 # attention with heads of 128: 228 registers, 196 with it).
 EXTRA_FLAGS = {"kq_mv_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
                "kv4_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
                "kv4_weigh.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
                "kv4_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+               "kv4_tree.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
                "w8_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
                "w8_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 

@@ -80,6 +80,11 @@ size_t kv4_attn_work_bytes(int head_dim);
 hipError_t launch_kv4_attn(int head_dim, const Kv4View& c, int type, const Kv4Rows& rows, const Kv4Attn& a,
                            hipStream_t s);
 
+// Attention of trees of drafted tokens (a.mask is set; kv4_tree.hip).
+size_t kv4_tree_work_bytes(int head_dim, int rows, int group);
+hipError_t launch_kv4_tree(int head_dim, const Kv4View& c, int type, const Kv4Rows& rows, const Kv4Attn& a,
+                           hipStream_t s);
+
 // Attention of many rows (kv4_prefill.hip), without a workspace.
 bool kv4_prefill_takes(const Kv4View& c, const Kv4Rows& rows, const Kv4Attn& a);
 hipError_t launch_kv4_prefill(int head_dim, const Kv4View& c, int type, const Kv4Rows& rows, const Kv4Attn& a,

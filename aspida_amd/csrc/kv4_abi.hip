@@ -251,8 +251,10 @@ extern "C" int aspida_tree_dev(const int* parent, int n_rows, int n_seq, const i
 
 extern "C" long long aspida_kv4_tree_attn_work_bytes(const aspida_kv4* cache, int n_heads, int n_rows, int n_seq,
                                                      int max_rows) {
-  if (max_rows > kq::TREE_MAX_ROWS) return -EINVAL;
-  return aspida_kv4_attn_work_bytes(cache, n_heads, n_rows, n_seq, max_rows);
+  if (!valid_cache(cache) || !valid_heads(cache, n_heads) || n_rows < 0 || n_seq < 0 || n_seq > 65535 || max_rows < 1 ||
+      max_rows > kq::TREE_MAX_ROWS)
+    return -EINVAL;
+  return (long long)kq::kv4_tree_work_bytes(cache->head_dim, longest(max_rows, n_rows), n_heads / cache->n_kv);
 }
 
 extern "C" int aspida_kv4_tree_attn_dev(const aspida_kv4* cache, int type, const void* q, long long q_stride,
@@ -273,7 +275,7 @@ extern "C" int aspida_kv4_tree_attn_dev(const aspida_kv4* cache, int type, const
   // Column tiles of all kv heads are a dimension of the launch.
   if (((long long)rows * (n_heads / cache->n_kv) + 15) / 16 * cache->n_kv > 65535) return -ENOTSUP;
   kq::Kv4Attn a{q, q_stride, out, out_stride, lse, work, n_heads, rows, window, scale, mask, mask_words};
-  return done(kq::launch_kv4_attn(cache->head_dim, view(cache), type, r, a, (hipStream_t)stream),
+  return done(kq::launch_kv4_tree(cache->head_dim, view(cache), type, r, a, (hipStream_t)stream),
               "aspida_kv4_tree_attn_dev");
 }
 

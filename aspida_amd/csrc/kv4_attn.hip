@@ -33,12 +33,12 @@
 // up to 8000 slots (bf16, 330 MB) 79 us, 4.2 TB/s.
 #include <algorithm>
 
-#include "kv4_mma.h"
+#include "kv4_split.h"
 
 namespace kq {
 
 constexpr int ATTN_WAVES = 4;
-constexpr int ATTN_STEP = 32 * ATTN_WAVES;  // tokens of a workgroup's round
+static_assert(ATTN_STEP == 32 * ATTN_WAVES);  // a workgroup's round
 // Tokens whose page ids a wave holds at once: whole rounds, within 64 pages
 // wherever in a page they start.
 constexpr int ATTN_SEGMENT = (4096 - 32) / ATTN_STEP * ATTN_STEP;
@@ -47,170 +47,6 @@ constexpr int ATTN_SEGMENT = (4096 - 32) / ATTN_STEP * ATTN_STEP;
 // measured against 1.5 and 2 rounds (32/8 heads, f32): 130001 slots 47, 59
 // and 57 us; 16 lanes of 8000 45, 56 and 54 us.
 template <int D> constexpr int ATTN_GROUPS = D == 64 ? 768 : D == 128 ? 512 : 256;
-constexpr float REF0 = -3.402823466e38f;  // below every score
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LN2 = 0.6931471805599453f;
-
-// Slots that a sequence's rows see together: [lo, hi), lo a multiple of 32.
-struct SeenRange { int lo, hi; };
-template <bool TREE>
-__device__ __forceinline__ SeenRange seen_range(const Kv4Span& s, int window, int max_slots) {
-  const int first = s.len - (s.r1 - s.r0);  // the first row's slot
-  SeenRange r;
-  r.hi = s.r1 > s.r0 ? min(s.len, max_slots) : 0;
-  const int lowest = TREE ? (window > 0 ? max(0, max(first, 0) - window) : 0) : kv4_lowest(first, kv4_reach(window));
-  r.lo = min(lowest, r.hi) & ~31;
-  return r;
-}
-
-// A sequence's rounds (one at least: one whose rows see nothing has outputs
-// too), and its length on the axis, which counts what a workgroup spends on a
-// sequence besides: its rows, page ids and sums, about 8000 cycles where a
-// round takes 1800.
-constexpr int AXIS_EXTRA = 4;
-template <bool TREE>
-__device__ __forceinline__ int rounds_of(const Kv4Span& s, int window, int max_slots) {
-  const SeenRange r = seen_range<TREE>(s, window, max_slots);
-  return max(1, (r.hi - r.lo + ATTN_STEP - 1) / ATTN_STEP);
-}
-
-// Where workgroup x's share starts: [x0, x0 + share) of the axis, sequence seq
-// (n_seq: none) from `start` of it on.
-struct AxisPlace { long long x0, share, start; int seq; };
-
-// Inclusive sum over the lanes.
-__device__ __forceinline__ long long wave_scan64(long long v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const long long u = __shfl_up(v, o, 64);
-    if (lane >= o) v += u;
-  }
-  return v;
-}
-
-// own: the span of sequence `lane`, which the first 64 sequences' lengths come
-// from.
-template <bool TREE>
-__device__ __forceinline__ long long axis_total(const Kv4Rows& rows, const Kv4Span& own, int window, int max_slots) {
-  const int lane = threadIdx.x & 63;
-  long long total = lane < rows.n_seq ? rounds_of<TREE>(own, window, max_slots) + AXIS_EXTRA : 0;
-  for (int b = 64 + lane; b < rows.n_seq; b += 64) total += rounds_of<TREE>(kv4_span(rows, b), window, max_slots) + AXIS_EXTRA;
-#pragma unroll
-  for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o, 64);
-  return total;
-}
-
-template <bool TREE>
-__device__ __forceinline__ AxisPlace axis_place(const Kv4Rows& rows, const Kv4Span& own, int window, int max_slots,
-                                                int groups, int x) {
-  const int lane = threadIdx.x & 63;
-  AxisPlace p;
-  if (rows.n_seq <= 64) {  // one lane each, and sums below 2^30
-    const int n = lane < rows.n_seq ? rounds_of<TREE>(own, window, max_slots) + AXIS_EXTRA : 0;
-    const int end = wave_scan_add(n);
-    p.share = (__builtin_amdgcn_readlane(end, 63) + groups - 1) / groups;
-    p.x0 = x * p.share;
-    const uint64_t over = __ballot(end > p.x0);
-    const int l = over ? __builtin_ctzll(over) : 63;
-    p.seq = over ? l : rows.n_seq;
-    p.start = __builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(n, l);
-    return p;
-  }
-  p.share = (axis_total<TREE>(rows, own, window, max_slots) + groups - 1) / groups;
-  p.x0 = x * p.share;
-  long long before = 0;
-  for (int b0 = 0; b0 < rows.n_seq; b0 += 64) {
-    const int b = b0 + lane;
-    const int n = b < rows.n_seq ? rounds_of<TREE>(b0 ? kv4_span(rows, b) : own, window, max_slots) + AXIS_EXTRA : 0;
-    const long long end = before + wave_scan64(n);
-    const uint64_t over = __ballot(end > p.x0);
-    if (over) {
-      const int l = __builtin_ctzll(over);
-      p.seq = b0 + l;
-      p.start = __shfl(end, l, 64) - __shfl(n, l, 64);
-      return p;
-    }
-    before = __shfl(end, 63, 64);
-  }
-  p.seq = rows.n_seq;
-  p.start = before;
-  return p;
-}
-
-// Workspace: per part, kv head and column tile the columns' sums [16][D] and
-// (ref, l) [16].  A workgroup has at most two sequences in part: one that
-// began in a share before its own (number 2 x) and one that goes on in the
-// next (2 x + 1), so parts number as the workgroups do, not as the sequences.
-template <int D> struct AttnPart {
-  float o[16][D];
-  float ref[16], l[16];
-};
-
-struct SplitArgs {
-  Kv4View c;
-  Kv4Rows rows;
-  Kv4Attn a;
-  int group, tiles;  // query heads of a kv head, column tiles
-  int groups;        // workgroups that share the axis
-};
-
-template <class T>
-__device__ __forceinline__ void store4(T* p, const float (&x)[4]) {
-  struct { T v[4]; } r;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r.v[i] = (T)x[i];
-  __builtin_memcpy(p, &r, sizeof(r));
-}
-
-// Rows past max_rows have no workgroup: NaN, by all threads of one.
-template <class T>
-__device__ void fill_excess(const SplitArgs& s, const Kv4Span& sp, int hk, int d) {
-  const int w = s.group * d;
-  for (int row = sp.r0 + s.a.max_rows; row < sp.r1; ++row) {
-    T* out = (T*)s.a.out + (size_t)row * s.a.out_stride + (size_t)hk * w;
-    for (int i = threadIdx.x; i < w; i += blockDim.x) out[i] = (T)__builtin_nanf("");
-    if (s.a.lse)
-      for (int i = threadIdx.x; i < s.group; i += blockDim.x)
-        s.a.lse[(size_t)row * s.a.n_heads + hk * s.group + i] = __builtin_nanf("");
-  }
-}
-
-// What a column of a tree sees: the slots [lo, base) and the rows [r0, r1)
-// that its mask names.
-struct TreeSeen {
-  const uint32_t* mask;
-  int lo, r0, r1;
-  __device__ __forceinline__ uint32_t word(int w) const {
-    uint32_t v = 32 * w < r1 && 32 * w + 32 > r0 ? mask[w] : 0u;
-    if (32 * w + 32 > r1) v &= r1 - 32 * w > 0 ? ~0u >> (32 * w + 32 - r1) : 0u;
-    if (32 * w < r0) v &= r0 - 32 * w < 32 ? ~0u << (r0 - 32 * w) : 0u;
-    return v;
-  }
-  // Bits of the rows j .. j + 31 (j may be below 0).
-  __device__ __forceinline__ uint32_t rows(int j) const {
-    const int w = j >> 5;
-    return __builtin_amdgcn_alignbit(word(w + 1), word(w), (uint32_t)(j & 31));
-  }
-  __device__ __forceinline__ TreeSeen() : mask(nullptr), lo(0), r0(0), r1(0) {}
-  // n rows at slots from base on, of which those at slots below 0 do not count.
-  __device__ __forceinline__ TreeSeen(const Kv4Attn& a, int row0, int row, int n, int base, bool valid) {
-    r0 = max(0, -base);
-    r1 = valid && base + row >= 0 ? min(n, 32 * a.mask_words) : 0;
-    mask = a.mask + (size_t)(row0 + (r1 > 0 ? row : 0)) * a.mask_words;
-    int shown = 0;
-    if (a.window > 0)
-      for (int w = 0; 32 * w < r1; ++w) shown += __popc(word(w));
-    lo = r1 <= 0 ? max(base, 0) : a.window > 0 ? max(0, max(base, 0) - max(a.window - shown, 0)) : 0;
-  }
-  // Whether it sees a slot from max_slots on.
-  __device__ __forceinline__ bool past(int base, int max_slots) const {
-    if (lo < base && base > max_slots) return true;
-    bool any = false;
-    for (int j = max(0, max_slots - base); j < r1; j += 32) any |= rows(j) != 0;
-    return any;
-  }
-};
 
 template <int D, class T, bool TREE>
 __global__ __launch_bounds__(64 * ATTN_WAVES, D == 64 ? 3 : D == 128 ? 2 : 1) void kv4_attn_split(SplitArgs s) {
@@ -453,75 +289,11 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, D == 64 ? 3 : D == 128 ? 2 : 1) vo
         s.a.lse[(size_t)(sp.r0 + row) * s.a.n_heads + head] = l != 0.f ? (ref + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
       continue;
     }
-    AttnPart<D>* part = (AttnPart<D>*)s.a.work + (2 * (size_t)blockIdx.x + (u0 == 0)) * gridDim.y + blockIdx.y;
+    AttnPart<D, 16>* part = (AttnPart<D, 16>*)s.a.work + (2 * (size_t)blockIdx.x + (u0 == 0)) * gridDim.y + blockIdx.y;
 #pragma unroll
     for (int i = 0; i < NT; ++i) *reinterpret_cast<kvf4*>(&part->o[col][16 * i + 4 * rg]) = o[i];
     if (rg == 0) { part->ref[col] = ref; part->l[col] = l; }
   }
-}
-
-// Joins the parts of a sequence: a workgroup per (column of a kv head's
-// tile, sequence).  Each of its waves takes every fourth part, 64 lanes over
-// the dims; LDS adds the four up.
-template <int D, class T, bool TREE>
-__global__ __launch_bounds__(256) void kv4_attn_join(SplitArgs s) {
-  constexpr int E = D / 64;
-  __shared__ float so[4][D], sl[4];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int b = blockIdx.z, hk = blockIdx.y / s.tiles, tile = blockIdx.y % s.tiles, col = blockIdx.x;
-  const Kv4Span sp = kv4_span(s.rows, b);
-  const int ncol = min(16, min(sp.r1 - sp.r0, s.a.max_rows) * s.group - tile * 16);
-  if (col >= ncol) return;
-  const int max_slots = s.c.max_pages * KV4_PAGE;
-  Kv4Span own = {0, 0, 0};
-  if (lane < s.rows.n_seq) own = kv4_span(s.rows, lane);
-  long long total, start;  // the axis, and where this sequence begins on it
-  if (s.rows.n_seq <= 64) {
-    const int n = lane < s.rows.n_seq ? rounds_of<TREE>(own, s.a.window, max_slots) + AXIS_EXTRA : 0;
-    const int upto = wave_scan_add(n);
-    total = __builtin_amdgcn_readlane(upto, 63);
-    start = __builtin_amdgcn_readlane(upto, b) - __builtin_amdgcn_readlane(n, b);
-  } else {
-    total = axis_total<TREE>(s.rows, own, s.a.window, max_slots);
-    start = lane < b ? rounds_of<TREE>(own, s.a.window, max_slots) + AXIS_EXTRA : 0;
-    for (int i = 64 + lane; i < b; i += 64)
-      start += rounds_of<TREE>(kv4_span(s.rows, i), s.a.window, max_slots) + AXIS_EXTRA;
-#pragma unroll
-    for (int o = 32; o; o >>= 1) start += __shfl_xor(start, o, 64);
-  }
-  const long long share = (total + s.groups - 1) / s.groups;
-  start += AXIS_EXTRA;
-  const long long first = start / share, last = (start + rounds_of<TREE>(sp, s.a.window, max_slots) - 1) / share;
-  const int count = (int)(last - first) + 1;
-  if (count == 1) return;
-  // Its parts: number 2 first + 1, then 2 x of the workgroups behind.
-  const size_t step = gridDim.y;
-  const AttnPart<D>* parts = (const AttnPart<D>*)s.a.work + 2 * (size_t)first * step + blockIdx.y;
-  auto part = [&](int i) -> const AttnPart<D>& { return parts[(i ? 2 * (size_t)i : 1) * step]; };
-  float ref = REF0;
-  for (int i = lane; i < count; i += 64) ref = fmaxf(ref, part(i).ref[col]);
-  for (int o = 32; o; o >>= 1) ref = fmaxf(ref, __shfl_xor(ref, o, 64));
-  float l = 0.f, y[E] = {};
-#pragma unroll 8
-  for (int i = wave; i < count; i += 4) {
-    const AttnPart<D>& p = part(i);
-    const float f = __builtin_amdgcn_exp2f(p.ref[col] - ref);
-    l += p.l[col] * f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) y[e] += p.o[col][lane * E + e] * f;
-  }
-#pragma unroll
-  for (int e = 0; e < E; ++e) so[wave][lane * E + e] = y[e];
-  if (lane == 0) sl[wave] = l;
-  __syncthreads();
-  const int i = threadIdx.x;
-  if (i >= D) return;
-  l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-  const float v = (so[0][i] + so[1][i]) + (so[2][i] + so[3][i]);
-  const int ci = tile * 16 + col, row = sp.r0 + ci / s.group, head = hk * s.group + ci % s.group;
-  ((T*)s.a.out)[(size_t)row * s.a.out_stride + (size_t)head * D + i] = (T)(l != 0.f ? v / l : 0.f);
-  if (s.a.lse && i == 0)
-    s.a.lse[(size_t)row * s.a.n_heads + head] = l != 0.f ? (ref + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
 }
 
 // (kv4_prefill_takes leaves at most 65535 of all kv heads.)
@@ -535,9 +307,9 @@ template <int D> static int attn_groups(int per_seq) { return std::max(1, ATTN_G
 // ATTN_GROUPS: with more tiles one workgroup walks the whole axis, and there
 // are no parts.
 size_t kv4_attn_work_bytes(int head_dim) {
-  return head_dim == 64    ? 2 * ATTN_GROUPS<64> * sizeof(AttnPart<64>)
-         : head_dim == 128 ? 2 * ATTN_GROUPS<128> * sizeof(AttnPart<128>)
-                           : 2 * ATTN_GROUPS<256> * sizeof(AttnPart<256>);
+  return head_dim == 64    ? 2 * ATTN_GROUPS<64> * sizeof(AttnPart<64, 16>)
+         : head_dim == 128 ? 2 * ATTN_GROUPS<128> * sizeof(AttnPart<128, 16>)
+                           : 2 * ATTN_GROUPS<256> * sizeof(AttnPart<256, 16>);
 }
 
 template <int D, class T, bool TREE>
@@ -546,7 +318,7 @@ static void attn_go(SplitArgs s, hipStream_t st) {
   s.groups = attn_groups<D>(per_seq);
   hipLaunchKernelGGL((kv4_attn_split<D, T, TREE>), dim3(s.groups, per_seq), dim3(64 * ATTN_WAVES), 0, st, s);
   const int cols = (int)std::min<long long>(16, (long long)s.a.max_rows * s.group);
-  hipLaunchKernelGGL((kv4_attn_join<D, T, TREE>), dim3(cols, per_seq, s.rows.n_seq), dim3(256), 0, st, s);
+  hipLaunchKernelGGL((kv4_attn_join<D, T, 16, TREE>), dim3(cols, per_seq, s.rows.n_seq), dim3(256), 0, st, s);
 }
 
 template <class T, bool TREE>
