@@ -85,46 +85,70 @@ __global__ __launch_bounds__(256) void tree_says(const T* logits, long long stri
   out[(size_t)row * pieces + piece] = s;
 }
 
-// A workgroup per sequence.
+// What a row says as a number that is larger for a larger logit, then for a
+// lower index; 0: nothing.
+__device__ __forceinline__ unsigned long long said_key(const Said& s) {
+  if (s.i == 0x7FFFFFFF) return 0;
+  const uint32_t u = __float_as_uint(s.v + 0.f);  // (-0 is 0)
+  return (unsigned long long)(u >> 31 ? ~u : u | 0x80000000u) << 32 | (uint32_t)~s.i;
+}
+__device__ __forceinline__ int said_token(unsigned long long key) { return key ? ~(int)(uint32_t)key : -1; }
+
+// A workgroup per sequence: every piece's key to its row's, every row that its
+// parent says to the parent's next, and a thread follows those.  (Atomics on
+// LDS whose result does not depend on their order.)
 __global__ __launch_bounds__(256) void tree_walk(TreeRows t, TreeAccept a, int pieces, int cap) {
-  extern __shared__ int lds[];  // says, token, parent of up to cap rows
-  __shared__ int found;
-  int *const says = lds, *const token = lds + cap, *const up = lds + 2 * cap;
+  extern __shared__ unsigned long long lds[];  // key and next row of up to cap rows
+  __shared__ int ends[2];                      // rows of the path, what the last one says
+  unsigned long long* const says = lds;
+  int* const next = (int*)(lds + cap);
   const int b = blockIdx.x, tid = threadIdx.x;
   const Kv4Span sp = kv4_span({t.row_start, t.kv_len, t.n_rows, t.n_seq}, b);
   const int n = sp.r1 - sp.r0, m = min(n, cap);
   const Said* const in = (const Said*)a.work + (size_t)sp.r0 * pieces;
+  const int total = m * pieces;  // below 2048 + 2 * 4096
+  Said u = {0.f, 0x7FFFFFFF};
+  int up = -1, token = -1;
+  if (tid < total) u = in[tid];
+  if (tid < m) {
+    up = tree_parent(t.parent + sp.r0, tid);
+    token = a.token[sp.r0 + tid];
+  }
   for (int i = tid; i < m; i += 256) {
-    Said s = {-INFINITY, 0x7FFFFFFF};
-    for (int p = 0; p < pieces; ++p) {
-      const Said u = in[(size_t)i * pieces + p];
-      say(s, u.v, u.i);
-    }
-    says[i] = s.i == 0x7FFFFFFF ? -1 : s.i;
-    token[i] = a.token[sp.r0 + i];
-    up[i] = tree_parent(t.parent + sp.r0, i);
+    says[i] = 0;
+    next[i] = m;
   }
-  int count = 0, said = -1;
-  for (int at = 0; at < m; ++count) {
-    if (tid == 0) {
-      found = m;
-      a.path[sp.r0 + count] = at;
-    }
-    __syncthreads();
-    said = says[at];
-    for (int i = at + 1 + tid; i < m; i += 256)
-      if (up[i] == at && token[i] == said && said >= 0) {
-        atomicMin(&found, i);
-        break;
-      }
-    __syncthreads();
-    at = found;
-    __syncthreads();
+  __syncthreads();
+  for (int x = tid; x < total;) {
+    atomicMax(&says[x / pieces], said_key(u));
+    x += 256;
+    if (x < total) u = in[x];
   }
+  __syncthreads();
+  for (int i = tid; i < m;) {
+    if (up >= 0 && token >= 0 && token == said_token(says[up])) atomicMin(&next[up], i);
+    i += 256;
+    if (i < m) {
+      up = tree_parent(t.parent + sp.r0, i);
+      token = a.token[sp.r0 + i];
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    int count = 0, last = 0;
+    for (int at = 0; at < m; at = next[at]) {
+      a.path[sp.r0 + count++] = at;
+      last = at;
+    }
+    ends[0] = count;
+    ends[1] = m > 0 ? said_token(says[last]) : -1;
+  }
+  __syncthreads();
+  const int count = ends[0];
   for (int i = count + tid; i < n; i += 256) a.path[sp.r0 + i] = -1;
   if (tid == 0) {
     a.count[b] = count;
-    a.next[b] = said;
+    a.next[b] = ends[1];
     a.new_len[b] = max(sp.len - n + count, 0);
   }
 }
@@ -153,7 +177,7 @@ hipError_t launch_tree_accept(int type, const TreeRows& t, const TreeAccept& a, 
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int cap = std::min(t.n_rows, TREE_MAX_ROWS);
-  hipLaunchKernelGGL(tree_walk, dim3(t.n_seq), dim3(256), 3 * sizeof(int) * cap, s, t, a, pieces, cap);
+  hipLaunchKernelGGL(tree_walk, dim3(t.n_seq), dim3(256), 12 * cap, s, t, a, pieces, cap);
   return hipGetLastError();
 }
 
