@@ -142,7 +142,7 @@ __global__ __launch_bounds__(256) void kv4_append(AppendArgs a) {
   __shared__ double freq[ROPE ? D / 2 : 1];
   __shared__ uint8_t vq[32][D];
   __shared__ int bad[32];  // the token's key or value holds a group that the format does not
-  const int b = blockIdx.z, tid = threadIdx.x;
+  const int b = blockIdx.y, tid = threadIdx.x;
   const Kv4Span sp = kv4_span(a.rows, b);
   const int n = sp.r1 - sp.r0, slot0 = sp.len - n;  // the first row's slot, below 0 where kv_len < n
   const int lo = max(slot0, 0), hi = min((long long)sp.len, (long long)a.c.max_pages * KV4_PAGE);
@@ -152,7 +152,7 @@ __global__ __launch_bounds__(256) void kv4_append(AppendArgs a) {
   auto angle = [](int p, int tok) { return 32 * p + 4 * (p >> 3) + tok; };
   if (ROPE && tid < half) freq[tid] = a.t.freq[tid];
   __syncthreads();
-  for (int blk = (lo >> 5) + blockIdx.x; blk <= (hi - 1) >> 5; blk += gridDim.x) {
+  for (int blk = (lo >> 5) + blockIdx.z; blk <= (hi - 1) >> 5; blk += gridDim.z) {
     uint8_t* page = kv4_block(a.c, b, blk >> 1, 0, L::BYTES);
     if (!page) continue;
     const int s0 = blk << 5, p0 = (blk & 1) * 32;  // first slot, and its token of the page
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(256) void kv4_append(AppendArgs a) {
         }
       }
     }
-    for (int hk = blockIdx.y; hk < a.c.n_kv; hk += gridDim.y) {
+    for (int hk = blockIdx.x; hk < a.c.n_kv; hk += gridDim.x) {
       uint8_t* base = page + (size_t)hk * L::BYTES;
       const T* k = (const T*)a.k + row * a.ks + (size_t)hk * D;
       const T* v = (const T*)a.v + row * a.vs + (size_t)hk * D;
@@ -293,12 +293,12 @@ struct ReadArgs {
 template <int D, class T>
 __global__ __launch_bounds__(256) void kv4_read(ReadArgs a) {
   using L = Kv4L<D>;
-  const int hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const int hk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const Kv4Span sp = kv4_span(a.rows, b);
   const int n = sp.r1 - sp.r0, slot0 = sp.len - n;
   const int lo = max(slot0, 0), hi = sp.len;
   if (n <= 0 || lo >= hi) return;
-  for (int blk = (lo >> 5) + blockIdx.x; blk <= (hi - 1) >> 5; blk += gridDim.x) {
+  for (int blk = (lo >> 5) + blockIdx.z; blk <= (hi - 1) >> 5; blk += gridDim.z) {
     const uint8_t* base = kv4_block(a.c, b, blk >> 1, hk, L::BYTES);
     const int s0 = blk << 5, p0 = (blk & 1) * 32;
     auto in = [&](int t) { return s0 + t >= lo && s0 + t < hi; };
@@ -351,7 +351,9 @@ __global__ __launch_bounds__(256) void kv4_read(ReadArgs a) {
 // Workgroups per (kv head, sequence): one for every 32-slot block of an
 // average sequence, and up to 4096 in all for longer ones, which otherwise take
 // theirs in turns (prompts of 4097, 1013 and 2 rows: 57 us with 55 of 128
-// blocks at a time).
+// blocks at a time).  They are the launch's last dimension: as its first, the
+// few that short sequences use fell on two of the XCDs (32 lanes of 5 to 26 rows,
+// 8 heads of 128, bf16, written and read back: 36 us, 11 now).
 static unsigned blocks_of(const Kv4Rows& r, int n_kv) {
   const long long most = r.n_rows / 32 + 2, mean = ((long long)r.n_rows + r.n_seq - 1) / r.n_seq / 32 + 2;
   const long long room = 4096 / ((long long)n_kv * r.n_seq);
@@ -365,7 +367,7 @@ static void append_go(const AppendArgs& a, bool rope, hipStream_t s) {
   // compute unit (7352 rows of 8 heads: one 34.7 us, two 33.8).
   const long long all = ((long long)a.rows.n_rows / 32 + a.rows.n_seq) * a.c.n_kv;
   const int turns = rope ? (int)std::min<long long>(std::max<long long>(all / 768, 1), a.c.n_kv) : 1;
-  const dim3 grid(blocks, (a.c.n_kv + turns - 1) / turns, a.rows.n_seq);
+  const dim3 grid((a.c.n_kv + turns - 1) / turns, a.rows.n_seq, blocks);
   if (!rope) hipLaunchKernelGGL((kv4_append<D, T, ROPE_NONE>), grid, dim3(256), 0, s, a);
   else if (a.t.interleaved || a.t.rot_dim % 16) hipLaunchKernelGGL((kv4_append<D, T, ROPE_ANY>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((kv4_append<D, T, ROPE_EIGHTS>), grid, dim3(256), 0, s, a);
@@ -397,7 +399,7 @@ hipError_t launch_kv4_append(int head_dim, const Kv4View& c, int type, const voi
 
 template <int D>
 static void read_typed(const ReadArgs& a, int type, hipStream_t s) {
-  const dim3 grid(blocks_of(a.rows, a.c.n_kv), a.c.n_kv, a.rows.n_seq);
+  const dim3 grid(a.c.n_kv, a.rows.n_seq, blocks_of(a.rows, a.c.n_kv));
   if (type == ACT_F32) hipLaunchKernelGGL((kv4_read<D, float>), grid, dim3(256), 0, s, a);
   else if (type == ACT_F16) hipLaunchKernelGGL((kv4_read<D, _Float16>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((kv4_read<D, bf16_t>), grid, dim3(256), 0, s, a);
