@@ -211,13 +211,17 @@ static hipError_t gemm_go(const W8Args& a, hipStream_t st) {
 // A token a workgroup, or four (64 bytes of a tile's line are written
 // together): from 2048 tokens on the latter is faster (bf16, 4096 inputs:
 // 1024 tokens 8.3 against 11.3 us, 2001 11.9 and 12.8, 4001 21.3 and 17.5;
-// 14336 inputs: 2001 31.6 and 32.4, 4001 56.8 and 49.2).
+// 14336 inputs: 2001 31.6 and 32.4, 4001 56.8 and 49.2).  Wide rows of tokens
+// that do not fill the card have four times the threads (product with 1024
+// rows, bf16, 14336 inputs, 256 and 1024 threads: 60 tokens 21.9 and 19.8 us,
+// 256 tokens 23.9 and 21.6, 512 tokens 31.9 and 33.2).
 template <class T> static void launch_tokens(const W8Args& a, hipStream_t st) {
-  auto go = [&](auto* k, int tok) {
-    hipLaunchKernelGGL(k, dim3((a.n_tok + tok - 1) / tok), dim3(256), 0, st, (const T*)a.x, a.x_stride, a.n_tok, a.in_dim, a.work);
+  auto go = [&](auto* k, int tok, int threads = 256) {
+    hipLaunchKernelGGL(k, dim3((a.n_tok + tok - 1) / tok), dim3(threads), 0, st, (const T*)a.x, a.x_stride, a.n_tok, a.in_dim, a.work);
   };
   if (a.n_tok >= 2048) go(&w8_tokens<T, 4, 256, 8 / (int)sizeof(T) == 4 ? 2 : 4>, 4);
   else if (a.in_dim <= 4096) go(&w8_tokens<T, 1, 256, 1>, 1);
+  else if (a.n_tok <= 256) go(&w8_tokens<T, 1, 1024, 1>, 1, 1024);
   else go(&w8_tokens<T, 1, 256, 4>, 1);
 }
 
