@@ -179,68 +179,4 @@ struct TreeSeen {
   }
 };
 
-// Joins the parts of a sequence: a workgroup per (column of a kv head's
-// tile, sequence).  Each of its waves takes every fourth part, 64 lanes over
-// the dims; LDS adds the four up.
-template <int D, class T, int COLS, bool TREE>
-__global__ __launch_bounds__(256) void kv4_attn_join(SplitArgs s) {
-  constexpr int E = D / 64;
-  __shared__ float so[4][D], sl[4];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int b = blockIdx.z, hk = blockIdx.y / s.tiles, tile = blockIdx.y % s.tiles, col = blockIdx.x;
-  const Kv4Span sp = kv4_span(s.rows, b);
-  const int ncol = min(COLS, min(sp.r1 - sp.r0, s.a.max_rows) * s.group - tile * COLS);
-  if (col >= ncol) return;
-  const int max_slots = s.c.max_pages * KV4_PAGE;
-  Kv4Span own = {0, 0, 0};
-  if (lane < s.rows.n_seq) own = kv4_span(s.rows, lane);
-  long long total, start;  // the axis, and where this sequence begins on it
-  if (s.rows.n_seq <= 64) {
-    const int n = lane < s.rows.n_seq ? rounds_of<TREE>(own, s.a.window, max_slots) + AXIS_EXTRA : 0;
-    const int upto = wave_scan_add(n);
-    total = __builtin_amdgcn_readlane(upto, 63);
-    start = __builtin_amdgcn_readlane(upto, b) - __builtin_amdgcn_readlane(n, b);
-  } else {
-    total = axis_total<TREE>(s.rows, own, s.a.window, max_slots);
-    start = lane < b ? rounds_of<TREE>(own, s.a.window, max_slots) + AXIS_EXTRA : 0;
-    for (int i = 64 + lane; i < b; i += 64)
-      start += rounds_of<TREE>(kv4_span(s.rows, i), s.a.window, max_slots) + AXIS_EXTRA;
-#pragma unroll
-    for (int o = 32; o; o >>= 1) start += __shfl_xor(start, o, 64);
-  }
-  const long long share = (total + s.groups - 1) / s.groups;
-  start += AXIS_EXTRA;
-  const long long first = start / share, last = (start + rounds_of<TREE>(sp, s.a.window, max_slots) - 1) / share;
-  const int count = (int)(last - first) + 1;
-  if (count == 1) return;
-  // Its parts: number 2 first + 1, then 2 x of the workgroups behind.
-  const size_t step = gridDim.y;
-  const AttnPart<D, COLS>* parts = (const AttnPart<D, COLS>*)s.a.work + 2 * (size_t)first * step + blockIdx.y;
-  auto part = [&](int i) -> const AttnPart<D, COLS>& { return parts[(i ? 2 * (size_t)i : 1) * step]; };
-  float ref = REF0;
-  for (int i = lane; i < count; i += 64) ref = fmaxf(ref, part(i).ref[col]);
-  for (int o = 32; o; o >>= 1) ref = fmaxf(ref, __shfl_xor(ref, o, 64));
-  float l = 0.f, y[E] = {};
-#pragma unroll 8
-  for (int i = wave; i < count; i += 4) {
-    const AttnPart<D, COLS>& p = part(i);
-    const float f = __builtin_amdgcn_exp2f(p.ref[col] - ref);
-    l += p.l[col] * f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) y[e] += p.o[col][lane * E + e] * f;
-  }
-#pragma unroll
-  for (int e = 0; e < E; ++e) so[wave][lane * E + e] = y[e];
-  if (lane == 0) sl[wave] = l;
-  __syncthreads();
-  const int i = threadIdx.x;
-  if (i >= D) return;
-  l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-  const float v = (so[0][i] + so[1][i]) + (so[2][i] + so[3][i]);
-  const int ci = tile * COLS + col, row = sp.r0 + ci / s.group, head = hk * s.group + ci % s.group;
-  ((T*)s.a.out)[(size_t)row * s.a.out_stride + (size_t)head * D + i] = (T)(l != 0.f ? v / l : 0.f);
-  if (s.a.lse && i == 0)
-    s.a.lse[(size_t)row * s.a.n_heads + head] = l != 0.f ? (ref + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
-}
-
 }  // namespace kq

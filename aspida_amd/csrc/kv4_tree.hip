@@ -366,6 +366,79 @@ __global__ __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) void kv4_tree(SplitAr
   }
 }
 
+// Joins the parts of a sequence, as kv4_attn_join does, but with a wave a
+// column: trees have hundreds of columns and few parts, and what a workgroup
+// spends on finding its parts is most of a join's time (16 trees of up to 104
+// columns and 8 kv heads: 19 us with a workgroup a column, 10 here).
+template <int D, class T, int COLS>
+__global__ __launch_bounds__(256) void kv4_tree_join(SplitArgs s) {
+  constexpr int E = D / 64;
+  struct Dims { float v[E]; };
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = blockIdx.z, hk = blockIdx.y / s.tiles, tile = blockIdx.y % s.tiles, col = 4 * blockIdx.x + wave;
+  const Kv4Span sp = kv4_span(s.rows, b);
+  const int ncol = min(COLS, min(sp.r1 - sp.r0, s.a.max_rows) * s.group - tile * COLS);
+  if (col >= ncol) return;
+  const int max_slots = s.c.max_pages * KV4_PAGE, length = rounds_of<true>(sp, s.a.window, max_slots);
+  int first, count;  // of the workgroups that share it
+  if (s.rows.n_seq <= 64) {  // (sums below 2^30)
+    int n = 0;
+    if (lane < s.rows.n_seq) n = rounds_of<true>(kv4_span(s.rows, lane), s.a.window, max_slots) + AXIS_EXTRA;
+    const int upto = wave_scan_add(n);
+    const uint32_t share = ((uint32_t)__builtin_amdgcn_readlane(upto, 63) + s.groups - 1) / (uint32_t)s.groups;
+    const uint32_t start = __builtin_amdgcn_readlane(upto, b) - length;
+    first = (int)(start / share);
+    count = (int)((start + length - 1) / share) - first + 1;
+  } else {
+    Kv4Span own = {0, 0, 0};
+    if (lane < s.rows.n_seq) own = kv4_span(s.rows, lane);
+    const long long share = (axis_total<true>(s.rows, own, s.a.window, max_slots) + s.groups - 1) / s.groups;
+    long long start = 0;
+    for (int i = lane; i < b; i += 64) start += rounds_of<true>(kv4_span(s.rows, i), s.a.window, max_slots) + AXIS_EXTRA;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) start += __shfl_xor(start, o, 64);
+    start += AXIS_EXTRA;
+    first = (int)(start / share);
+    count = (int)((start + length - 1) / share) - first + 1;
+  }
+  if (count == 1) return;
+  // Its parts: number 2 first + 1, then 2 x of the workgroups behind.
+  const size_t step = gridDim.y;
+  const AttnPart<D, COLS>* parts = (const AttnPart<D, COLS>*)s.a.work + 2 * (size_t)first * step + blockIdx.y;
+  auto part = [&](int i) -> const AttnPart<D, COLS>& { return parts[(i ? 2 * (size_t)i : 1) * step]; };
+  float ref = REF0;
+  for (int i = lane; i < count; i += 64) ref = fmaxf(ref, part(i).ref[col]);
+#pragma unroll
+  for (int o = 32; o; o >>= 1) ref = fmaxf(ref, __shfl_xor(ref, o, 64));
+  float l = 0.f, y[E] = {};
+  for (int c0 = 0; c0 < count; c0 += 64) {
+    const int here = min(count - c0, 64);
+    const AttnPart<D, COLS>& own = part(c0 + min(lane, here - 1));
+    const float f = lane < here ? __builtin_amdgcn_exp2f(own.ref[col] - ref) : 0.f;
+    if (lane < here) l += own.l[col] * f;
+    for (int i = 0; i < here; i += 8) {  // (past the last part it is the last one again, with a weight of 0)
+      Dims o[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        o[j] = *reinterpret_cast<const Dims*>(&part(c0 + min(i + j, here - 1)).o[col][lane * E]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float fj = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i + j));
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = __builtin_fmaf(o[j].v[e], fj, y[e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o, 64);
+  const int ci = tile * COLS + col, row = sp.r0 + ci / s.group, head = hk * s.group + ci % s.group;
+  T* out = (T*)s.a.out + (size_t)row * s.a.out_stride + (size_t)head * D + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) out[e] = (T)(l != 0.f ? y[e] / l : 0.f);
+  if (s.a.lse && lane == 0)
+    s.a.lse[(size_t)row * s.a.n_heads + head] = l != 0.f ? (ref + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+}
+
 // Workgroups that fit at once: one of eight waves a compute unit, two of four
 // (one for heads of 256, whose stages take 103 KB).
 template <int D, int WAVES> constexpr int TREE_ROOM = WAVES == 4 && D != 256 ? 512 : 256;
@@ -384,7 +457,7 @@ static hipError_t tree_go(SplitArgs s, hipStream_t st) {
   s.groups = std::max(1, TREE_ROOM<D, WAVES> / per_seq);
   hipLaunchKernelGGL((kv4_tree<D, T, WAVES>), dim3(s.groups, per_seq), dim3(64 * WAVES), lds, st, s);
   if (s.groups > 1)
-    hipLaunchKernelGGL((kv4_attn_join<D, T, 32 * WAVES, true>), dim3((unsigned)std::min<long long>(32 * WAVES, cols), per_seq, s.rows.n_seq), dim3(256), 0, st, s);
+    hipLaunchKernelGGL((kv4_tree_join<D, T, 32 * WAVES>), dim3((unsigned)(std::min<long long>(32 * WAVES, cols) + 3) / 4, per_seq, s.rows.n_seq), dim3(256), 0, st, s);
   return hipGetLastError();
 }
 

@@ -57,14 +57,9 @@ hipError_t launch_w8(int type, const W8Args& a, hipStream_t s);
 
 #ifdef __HIPCC__
 typedef int w8i4 __attribute__((ext_vector_type(4)));
-typedef int w8i16 __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ w8i4 w8_mfma(w8i4 a, w8i4 b, w8i4 c) {
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
-}
-
-__device__ __forceinline__ w8i16 w8_mfma32(w8i4 a, w8i4 b, w8i16 c) {
-  return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
 }
 
 // A row's scale from its largest magnitude (NaN where a value is not finite:

@@ -9,8 +9,8 @@ import aspida_amd as aa
 import kv4_plain
 import more_plain as plain
 import test_gpu_tree as tree
-from gpu_helpers import torch_cuda
-from test_gpu_kv4 import NAMES, Cache, _dev, _filled, _kv, _starts
+from gpu_helpers import stream, torch_cuda
+from test_gpu_kv4 import NAMES, Cache, _dev, _filled, _i32, _kv, _starts
 from test_gpu_tree import SHARES, TREES, _check_tree, _forest, _tree_attend
 
 pytestmark = pytest.mark.gpu
@@ -131,3 +131,42 @@ def test_unseen_slots_never_matter_and_seen_ones_always(ty, dim):
     assert torch.isnan(o5[16:]).all()
     o7, _ = _tree_attend(c, ty, q, [0, r], [pages * 64 + 1 + r], heads, 0.1, mask(np.zeros((r, r), bool)), 1)
     assert torch.isnan(o7).all()
+
+
+def test_captured_and_replayed():
+    """One launch list for lengths and masks that change between replays, with other work in between."""
+    torch = torch_cuda()
+    gen = np.random.default_rng(3)
+    rows, lens, heads = [40, 0, 25], [3000, 70, 5000], 16
+    c = _widen(_filled(gen, 128, 2, [n + 200 for n in lens]), 320)
+    starts = _starts(rows)
+    q = _dev(gen.standard_normal((65, heads * 128)).astype(np.float32), aa.BF16)
+    st, ln = _i32(starts), _i32(lens)
+    mask = torch.zeros((65, 2), dtype=torch.int32, device="cuda")
+    out, lse = torch.zeros_like(q), torch.zeros((65, heads), device="cuda")
+    work = torch.empty(c.dev.kv4_tree_attention_work_bytes(c.c, heads, 65, 3, 40), dtype=torch.uint8, device="cuda")
+    side = torch.cuda.Stream()
+
+    def run():
+        c.dev.kv4_tree_attention(c.c, aa.BF16, q.data_ptr(), heads * 128, heads, 65, 3, st.data_ptr(), 40, ln.data_ptr(),
+                                 mask.data_ptr(), 2, 0.1, out.data_ptr(), heads * 128, work.data_ptr(), stream(),
+                                 lse=lse.data_ptr())
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        run()
+    for turn in range(4):
+        now = [n + 50 * turn for n in lens]
+        ons = [plain.ancestors(_forest(gen, r)) for r in rows]
+        mask.copy_(_dev(np.concatenate([plain.mask_words(on, 2) if len(on) else np.zeros((0, 2), np.uint32) for on in ons]).view(np.int32)))
+        ln.copy_(_i32(now))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        a, la = out.clone(), lse.clone()
+        out.zero_()
+        run()
+        torch.cuda.synchronize()
+        assert torch.equal(a, out) and torch.equal(la, lse)
+        _check_tree(c, aa.BF16, q, starts, now, heads, 0.1, ons, 0, a, la)

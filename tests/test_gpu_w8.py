@@ -297,3 +297,10 @@ def test_captured_into_a_graph_and_on_two_streams(n):
     for o, (a, b) in zip(outs, want):
         for c, d in o:
             assert torch.equal(c, a) and torch.equal(d, b)
+
+
+@pytest.mark.parametrize("ty", [aa.F32, aa.BF16, aa.F16], ids=NAMES.get)
+@pytest.mark.parametrize("size", [(3, 4097, 20, 0), (60, 5003, 33, 1), (256, 4111, 17, 0), (257, 4111, 17, 0),
+                                  (7, 16385, 40, 3), (33, 40007, 5, 0)], ids=lambda s: f"t{s[0]}i{s[1]}o{s[2]}p{s[3]}")
+def test_odd_wide_rows_of_few_tokens(size, ty):
+    test_product(size, ty)
