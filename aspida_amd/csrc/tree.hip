@@ -5,8 +5,9 @@
 // equals (NaN never is one).  From row 0 on, the next row is the first child
 // whose token is what its parent says; where there is none, that is the next
 // token.  tree_says finds each row's largest in pieces (memory bound: all
-// logits are read once), tree_walk joins the pieces of a sequence's rows and
-// walks in LDS.
+// logits are read once; 254 rows of 151936, bf16, 77 MB in 17 us, 4.5 TB/s),
+// tree_walk joins the pieces of a sequence's rows and walks in LDS (2 to 4 us
+// behind a launch: bound by waiting).
 #include <algorithm>
 
 #include "kq_common.h"
@@ -106,7 +107,7 @@ __global__ __launch_bounds__(256) void tree_walk(TreeRows t, TreeAccept a, int p
   const Kv4Span sp = kv4_span({t.row_start, t.kv_len, t.n_rows, t.n_seq}, b);
   const int n = sp.r1 - sp.r0, m = min(n, cap);
   const Said* const in = (const Said*)a.work + (size_t)sp.r0 * pieces;
-  const int total = m * pieces;  // below 2048 + 2 * 4096
+  const int total = m * pieces;  // at most 4096
   Said u = {0.f, 0x7FFFFFFF};
   int up = -1, token = -1;
   if (tid < total) u = in[tid];
@@ -153,9 +154,10 @@ __global__ __launch_bounds__(256) void tree_walk(TreeRows t, TreeAccept a, int p
   }
 }
 
-// Pieces of a row: about 2048 workgroups in all, of at least 4096 elements.
+// Pieces of a row, of 4096 elements at least: 2048 workgroups in all at most,
+// which is what fits at once (254 rows of 151936, bf16: in 9 pieces 21.1 us, in 8 19.8).
 static int says_pieces(int n_rows, int vocab) {
-  return (int)std::max<long long>(1, std::min<long long>((2048 + n_rows - 1) / n_rows, (vocab + 4095) / 4096));
+  return (int)std::max<long long>(1, std::min<long long>(2048 / n_rows, (vocab + 4095) / 4096));
 }
 
 size_t tree_accept_work_bytes(int n_rows, int vocab) {
