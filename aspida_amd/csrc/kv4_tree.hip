@@ -16,11 +16,12 @@
 // the parts of a sequence.
 //
 // Bound by waiting at the barrier of every stage and for its data (45% of wave
-// time; vector units 50% busy, matrix cores 43%): 256 columns behind 32000 slots (32/8 heads of 128, bf16) take
-// 83 us, 404 TFLOP/s of the products that the formula has; the two planes of P
-// and the minima make 1.6 times as many.  In tiles of 16 columns, which unpack
-// every slot 16 times: 124 us; in tiles of 32 and 64 columns unpacked straight
-// into registers, which leave a wave a SIMD: 157 and 102 us.
+// time; vector units 50% busy, matrix cores 43%): 256 columns behind 32000
+// slots (32/8 heads of 128, bf16) take 83 us, 404 TFLOP/s of the products that
+// the formula has; the two planes of P and the minima make 1.6 times as many.
+// In tiles of 16 columns, which unpack every slot 16 times: 124 us; in tiles of
+// 32 and 64 columns unpacked straight into registers: 157 us (two waves a SIMD,
+// registers spilled) and 102 (one wave).
 #include <algorithm>
 
 #include "kv4_split.h"

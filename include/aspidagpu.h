@@ -375,8 +375,10 @@ int aspida_tree_dev(const int *parent, int n_rows, int n_seq, const int *row_sta
  * slots in all: the rows that its mask names, and as many of the last slots
  * before base as remain.  A row that sees nothing gets 0, and lse -inf; rows
  * at slots below 0 see nothing and are not seen.  max_rows (up to 4096) as
- * there.  -ENOTSUP for more than 65535 tiles of 16 columns (max_rows * heads of
- * a kv head) in all kv heads. */
+ * there.  work: 256-byte aligned, aspida_kv4_tree_attn_work_bytes for these
+ * arguments or larger ones: 6 to 9 MB, or up to 68 MB where max_rows * heads of
+ * a kv head is above 64.  -ENOTSUP for more than 65535 tiles of 16 columns
+ * (max_rows * heads of a kv head) in all kv heads. */
 long long aspida_kv4_tree_attn_work_bytes(const aspida_kv4 *cache, int n_heads, int n_rows, int n_seq, int max_rows);
 int aspida_kv4_tree_attn_dev(const aspida_kv4 *cache, int type, const void *q, long long q_stride, int n_heads,
                              int n_rows, int n_seq, const int *row_start, int max_rows, const int *kv_len,
